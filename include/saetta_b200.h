@@ -485,6 +485,114 @@ int saetta_att_gemm_partial_shard(saetta_att_gemm *op, const void *q_dev, int dt
                                   float *part_dev, saetta_flash_params p, size_t key_base,
                                   size_t key_lo, size_t key_hi, void *stream);
 
+/* ------------------------------------------------------------------ paged 8-bit cache
+ * For serving many requests: the cache of all of them is one pool of blocks of 16, 32,
+ * 64 or 128 tokens, a request owns the blocks that its row of the block table names, and
+ * a step's launches (assign, store, attend) take every length, table and slot from device
+ * memory, so that a captured graph of a step replays for any lengths.  No counterpart in
+ * the reference, whose caches are one contiguous buffer per sequence
+ * (src/gpu_layers.rs:179-293).
+ *
+ * Values are e4m3 with one scale for each (block, kv head, side), a power of two: within
+ * e4m3's range (18 powers of two) the scale costs no precision, and a block's scale can grow
+ * with the rows appended to it without rounding again what it holds, but for values that
+ * fall among e4m3's subnormals (below 2^-15 of the block's largest).  Head dim 128 or 256,
+ * 1 to 16 query heads per kv head.
+ *   keys, values  e4m3 [blocks][kv_heads][block_tokens][head_dim]
+ *   scales        f32  [blocks][kv_heads][2]  (of the keys, of the values); attend takes any
+ *                      finite scale >= 0, not only those that store writes
+ */
+typedef struct saetta_paged_cache saetta_paged_cache;
+int saetta_paged_cache_create(int device, size_t kv_heads, size_t head_dim, size_t block_tokens,
+                              size_t blocks, saetta_paged_cache **out);
+/* Over buffers of the caller's (16-byte aligned), which outlive the handle. */
+int saetta_paged_cache_wrap(int device, size_t kv_heads, size_t head_dim, size_t block_tokens,
+                            size_t blocks, void *keys_dev, void *values_dev, float *scales_dev,
+                            saetta_paged_cache **out);
+void saetta_paged_cache_destroy(saetta_paged_cache *cache);
+int saetta_paged_cache_buffers(const saetta_paged_cache *cache, void **keys_dev, void **values_dev,
+                               float **scales_dev);
+
+/* What the *status words of assign and store hold (0: all done). */
+#define SAETTA_PAGED_NO_BLOCKS 1u  /* more blocks are needed than the free stack holds */
+#define SAETTA_PAGED_TABLE_FULL 2u /* a sequence outgrows its row of the block table */
+#define SAETTA_PAGED_ROWS_FULL 4u  /* more new tokens than rows_cap */
+#define SAETTA_PAGED_BAD_SLOT 8u   /* store: a slot outside the cache or out of order; that row is not written */
+
+/* One scheduling step for `seqs` sequences (at most 8192), in one launch.  Sequence s holds
+ * kv_lens[s] tokens and gets new_tokens[s] more; where finished[s] is not 0 (finished_dev may
+ * be NULL) its blocks are first put on top of the free stack, in sequence and table order,
+ * and it starts over at length 0, so a new request may take its row in the same step.  Then
+ * blocks are taken from the top of the stack (free_blocks[free_count - 1] first), in
+ * sequence and table order, and written to block_tables [seqs][table_stride].
+ *   row_starts [seqs + 1]  first row of each sequence's new tokens, and their total
+ *   slots [rows_cap]       block * block_tokens + offset of each row; -1 behind the last
+ *   positions [rows_cap]   position of each row in its sequence; -1 behind the last; may be NULL
+ *   kv_lens_out [seqs], free_count_out   lengths and stack height after the step; may be the
+ *                          same addresses as kv_lens_dev and free_count_dev
+ *   status                 0, or SAETTA_PAGED_* bits: then nothing was assigned or given back,
+ *                          every slot is -1, row_starts are 0 and the lengths as they were, so
+ *                          the step's other launches find nothing to do
+ * free_cap: entries of free_blocks_dev (the number of blocks of the pool is enough). */
+int saetta_paged_assign(int device, size_t seqs, size_t block_tokens, const uint32_t *kv_lens_dev,
+                        const uint32_t *new_tokens_dev, const uint32_t *finished_dev,
+                        int32_t *free_blocks_dev, size_t free_cap, const uint32_t *free_count_dev,
+                        int32_t *block_tables_dev, size_t table_stride, uint32_t *row_starts_dev,
+                        int32_t *slots_dev, int32_t *positions_dev, size_t rows_cap,
+                        uint32_t *kv_lens_out_dev, uint32_t *free_count_out_dev,
+                        uint32_t *status_dev, void *stream);
+
+/* Appends rows [rows][kv_heads][head_dim] of k and v (dtype SAETTA_F32, SAETTA_F16 or
+ * SAETTA_BF16; k_stride, v_stride: values between rows; rows 16-byte aligned) at `slots`; a
+ * negative slot is skipped.  Rows of one block stand next to each other in rising order, as
+ * assign lays them out, and a slot occurs once: a row of the same block as the one before it
+ * but not its successor is not written and reported, as is a slot outside the cache
+ * (SAETTA_PAGED_BAD_SLOT is OR-ed into *status_dev, which may be NULL).  Two runs of rows in
+ * one block, apart from one another, leave that block undefined.
+ * A run that begins at a block's first token starts its scales anew from the run's values; a
+ * later one raises them where its values need it and re-scales the tokens before the run.
+ * Values are rounded to nearest even; infinities saturate, NaN stays NaN, and neither takes
+ * part in the scale. */
+int saetta_paged_store(saetta_paged_cache *cache, const void *k_dev, const void *v_dev, int dtype,
+                       size_t rows, size_t k_stride, size_t v_stride, const int32_t *slots_dev,
+                       uint32_t *status_dev, void *stream);
+
+/* The rows and keys of one attention call.  Sequence s has the query rows row_starts[s] ..
+ * row_starts[s + 1] - 1 of `rows`, and kv_lens[s] keys, its own rows' among them (store comes
+ * before attend): row i of n sees keys 0 .. kv_len - n + i.  A row that sees no key gets
+ * zeros; rows of no sequence are left as they were. */
+typedef struct saetta_paged_batch {
+    size_t seqs;         /* at most 8192 */
+    size_t rows;         /* rows of q and out */
+    size_t max_rows;     /* rows of the longest sequence at most: which kernel runs goes by it */
+    size_t table_stride; /* columns of the block tables */
+    const uint32_t *row_starts_dev;    /* [seqs + 1] */
+    const uint32_t *kv_lens_dev;       /* [seqs] */
+    const int32_t *block_tables_dev;   /* [seqs][table_stride] */
+} saetta_paged_batch;
+
+/* The op's workspace serves one call at a time: calls through one op follow one another on
+ * a stream (or are ordered by events); calls that overlap, two graphs replayed at once among
+ * them, need an op each. */
+typedef struct saetta_paged_attention saetta_paged_attention;
+int saetta_paged_attention_create(int device, size_t heads, size_t kv_heads, size_t head_dim,
+                                  saetta_paged_attention **out);
+void saetta_paged_attention_destroy(saetta_paged_attention *op);
+/* out [rows][heads][head_dim] = softmax(scale q K^T) V, times sigmoid(gate) where
+ * q_and_gate_dev (f32 [rows][heads][2 head_dim], the gate behind q) is not NULL.  q
+ * [rows][heads][head_dim], q_stride values between rows (at least heads * head_dim), rows
+ * 16-byte aligned; q_dtype and out_dtype each SAETTA_F32, SAETTA_F16 or SAETTA_BF16.
+ * Scores, sums and accumulators are f32; the products take q with the precision of its type,
+ * 11 bits of an f32 one, and the probabilities with 11 bits (8 for long bfloat16 chunks). */
+int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *cache,
+                        saetta_paged_batch batch, const void *q_dev, int q_dtype, size_t q_stride,
+                        const float *q_and_gate_dev, void *out_dev, int out_dtype, float scale,
+                        void *stream);
+/* The op's device status word: 0, or bits of a bounded wait that gave up (1, 2, 4: make a new
+ * op) or of a block table entry outside the cache (16: that block's keys were left out).
+ * Synchronises the stream. */
+int saetta_paged_attention_status(saetta_paged_attention *op, void *stream, uint32_t *status);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,7 @@ F16, BF16, F32 = 0, 1, -1
 KV_ALIGN = 128
 MAX_ROWS = 8
 PART_STRIDE = 264
+PAGED_NO_BLOCKS, PAGED_TABLE_FULL, PAGED_ROWS_FULL, PAGED_BAD_SLOT = 1, 2, 4, 8
 OK, BAD_ARG, BAD_SHAPE, NO_MEM, CUDA, TIMEOUT, UNSUPPORTED = range(7)
 
 
@@ -64,6 +65,12 @@ def build(verbose=False):
     cmd = ["make", "-C", os.path.join(_HERE, "csrc"), "-j8"]
     subprocess.check_call(cmd, stdout=None if verbose else subprocess.DEVNULL)
     return LIB_PATH
+
+
+class PagedBatch(C.Structure):
+    """The rows and keys of one paged attention call (no reference counterpart)."""
+    _fields_ = [("seqs", C.c_size_t), ("rows", C.c_size_t), ("max_rows", C.c_size_t), ("table_stride", C.c_size_t),
+                ("row_starts", C.c_void_p), ("kv_lens", C.c_void_p), ("block_tables", C.c_void_p)]
 
 
 _lib = None
@@ -158,6 +165,16 @@ SYMBOLS = {
     "saetta_att_gemm_partial": (_I, [_P, _P, _I, _P, _P, _P, _P, _P, FlashParams, _Z, _Z, _P]),
     "saetta_prefill_encode": (_I, [_I, _P, _I, _P, _P, _P, _P, FlashParams, _P]),
     "saetta_prefill_rows_cache": (_I, [_P, _P, _P, _P, _P, FlashParams, _P, _P]),
+    "saetta_paged_cache_create": (_I, [_I, _Z, _Z, _Z, _Z, _PP]),
+    "saetta_paged_cache_wrap": (_I, [_I, _Z, _Z, _Z, _Z, _P, _P, _P, _PP]),
+    "saetta_paged_cache_destroy": (None, [_P]),
+    "saetta_paged_cache_buffers": (_I, [_P, _PP, _PP, _PP]),
+    "saetta_paged_assign": (_I, [_I, _Z, _Z, _P, _P, _P, _P, _Z, _P, _P, _Z, _P, _P, _P, _Z, _P, _P, _P, _P]),
+    "saetta_paged_store": (_I, [_P, _P, _P, _I, _Z, _Z, _Z, _P, _P, _P]),
+    "saetta_paged_attention_create": (_I, [_I, _Z, _Z, _Z, _PP]),
+    "saetta_paged_attention_destroy": (None, [_P]),
+    "saetta_paged_attend": (_I, [_P, _P, PagedBatch, _P, _I, _Z, _P, _P, _I, C.c_float, _P]),
+    "saetta_paged_attention_status": (_I, [_P, _P, C.POINTER(_U32)]),
 }
 
 
@@ -685,6 +702,83 @@ def prefill_encode(device, q, keys, values, q_and_gate, out, p, dtype=F16, strea
     """src/attention_prefill.rs:39-72 `encode` (binary16 q and cache, as the reference's)."""
     _check(lib().saetta_prefill_encode(device, ptr(q), dtype, ptr(keys), ptr(values), ptr(q_and_gate), ptr(out), p,
                                        _stream(stream)))
+
+
+class PagedKvCache:
+    """A pool of blocks of e4m3 keys and values, one scale for each (block, kv head, side), that many sequences
+    share through block tables (no reference counterpart; layouts in include/saetta_b200.h)."""
+
+    def __init__(self, device, kv_heads, head_dim, block_tokens, blocks, _handle=None):
+        self.device, self.kv_heads, self.head_dim = device, kv_heads, head_dim
+        self.block_tokens, self.blocks = block_tokens, blocks
+        if _handle is None:
+            h = C.c_void_p()
+            _check(lib().saetta_paged_cache_create(device, kv_heads, head_dim, block_tokens, blocks, C.byref(h)))
+            _handle = h
+        self.h = _handle
+
+    @classmethod
+    def wrap(cls, device, kv_heads, head_dim, block_tokens, blocks, keys, values, scales):
+        h = C.c_void_p()
+        _check(lib().saetta_paged_cache_wrap(device, kv_heads, head_dim, block_tokens, blocks, ptr(keys), ptr(values),
+                                             ptr(scales), C.byref(h)))
+        c = cls(device, kv_heads, head_dim, block_tokens, blocks, _handle=h)
+        c._keep = (keys, values, scales)
+        return c
+
+    def buffers(self):
+        """Device addresses of (keys, values, scales)."""
+        k, v, s = C.c_void_p(), C.c_void_p(), C.c_void_p()
+        _check(lib().saetta_paged_cache_buffers(self.h, C.byref(k), C.byref(v), C.byref(s)))
+        return k.value, v.value, s.value
+
+    def store(self, k, v, slots, rows, dtype=F32, k_stride=None, v_stride=None, status=None, stream=None):
+        """Appends `rows` rows at `slots` (negative: skipped), as paged_assign lays them out."""
+        row = self.kv_heads * self.head_dim
+        _check(lib().saetta_paged_store(self.h, ptr(k), ptr(v), dtype, rows, row if k_stride is None else k_stride,
+                                        row if v_stride is None else v_stride, ptr(slots), ptr(status), _stream(stream)))
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.saetta_paged_cache_destroy(self.h)
+            self.h = None
+
+
+def paged_assign(device, seqs, block_tokens, kv_lens, new_tokens, free_blocks, free_cap, free_count, block_tables,
+                 table_stride, row_starts, slots, positions, rows_cap, kv_lens_out, free_count_out, status, finished=None,
+                 stream=None):
+    """One scheduling step: finished sequences give their blocks back, growing ones take blocks; tables, slots and
+    positions of the new rows (all 32-bit integers on the device)."""
+    _check(lib().saetta_paged_assign(device, seqs, block_tokens, ptr(kv_lens), ptr(new_tokens), ptr(finished),
+                                     ptr(free_blocks), free_cap, ptr(free_count), ptr(block_tables), table_stride,
+                                     ptr(row_starts), ptr(slots), ptr(positions), rows_cap, ptr(kv_lens_out),
+                                     ptr(free_count_out), ptr(status), _stream(stream)))
+
+
+class PagedAttention:
+    """Causal attention of ragged query rows (single tokens, verify rows, prompts) over a PagedKvCache."""
+
+    def __init__(self, device, heads, kv_heads, head_dim):
+        h = C.c_void_p()
+        _check(lib().saetta_paged_attention_create(device, heads, kv_heads, head_dim, C.byref(h)))
+        self.h, self.heads, self.head_dim = h, heads, head_dim
+
+    def record(self, cache, q, q_dtype, rows, seqs, row_starts, kv_lens, block_tables, table_stride, max_rows, scale, out,
+               out_dtype, q_and_gate=None, q_stride=None, stream=None):
+        batch = PagedBatch(seqs, rows, max_rows, table_stride, ptr(row_starts), ptr(kv_lens), ptr(block_tables))
+        _check(lib().saetta_paged_attend(self.h, cache.h, batch, ptr(q), q_dtype,
+                                         self.heads * self.head_dim if q_stride is None else q_stride, ptr(q_and_gate),
+                                         ptr(out), out_dtype, scale, _stream(stream)))
+
+    def device_status(self, stream=None):
+        s = C.c_uint32()
+        _check(lib().saetta_paged_attention_status(self.h, _stream(stream), C.byref(s)))
+        return s.value
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.saetta_paged_attention_destroy(self.h)
+            self.h = None
 
 
 def quantize_host(x, bits):

@@ -1,0 +1,471 @@
+// Attention of few rows (single tokens, verify rows) over the paged e4m3 cache.
+//
+//   s_ij = scale (q_i . kcode_j) ks[block(j)],  out_i = sum_j p_ij vs[block(j)] vcode_j / sum_j p_ij,  p = exp(s - max)
+//
+// A block's scales leave the products: they multiply a score, and a probability, of a whole block, so the codes go to the
+// tensor cores as they are (an e4m3 value is a binary16 value).  Bound by the cache's bytes, 2 * head_dim for each key and
+// kv head; the rest is arranged so that these stream without a pause:
+//
+//  * One CTA for each SM takes an equal share of all key tiles (paged_sched.cuh); a producer warp keeps a ring of
+//    64-key tiles of K and V in flight (TMA tensor copies of whole pages, 128-byte swizzle: 160 KB on the way with
+//    head dim 256) and the pages' scales beside them (8-byte asynchronous copies).
+//  * Eight consumer warps, four for each tile, 16 keys a warp, each with its own running maximum, sum and accumulators: no
+//    barrier between tiles.  Keys are the 16 rows of mma.m16n8k16, query rows its 8 columns (a group of 8 heads fills them).
+//    The order of dims inside a product is free, so a lane feeds 16 consecutive bytes of a key to four products; with the
+//    swizzle, chunk 2 t + j for lane t of a key makes these 128-bit loads free of bank conflicts, and chunk g for lane
+//    group g those of the values.
+//  * Values enter as pairs of keys of one dim: two byte permutes for four dims, then the conversion to binary16.
+//  * P is rounded to binary16 (11 bits; p times the value scale relative to the largest of the warp's so far), scores, sums
+//    and accumulators are f32.  Queries enter as binary16 after a power of two for each row, so bfloat16's range
+//    fits; f32 queries are rounded to 11 bits there.
+#include <algorithm>
+
+#include "paged_sched.cuh"
+#include "umma.cuh"
+
+namespace saetta {
+
+constexpr int kPdTile = 64;      // keys of a tile
+constexpr int kPdThreads = 288;  // 8 consumer warps, 1 producer warp
+constexpr float kPdRescale = 8.f; // the accumulators follow the running maximum only past this many doublings
+
+template <int D, int NT>
+struct PdLayout {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kSide = kPdTile * D;
+    static constexpr int kStage = 2 * kSide;
+    static constexpr int kStages = D == 256 ? 5 : 8;
+    static constexpr int kRow = 128 + 4;                      // floats of one row of the exchange buffer
+    static constexpr int kExchange = 8 * 8 * kRow * 4;        // 8 warps x 8 rows of 128 dims
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * 4 * 8 /*scales*/ + 3072 /*barriers, statistics*/;
+};
+static_assert(PdLayout<256, 2>::kSmem <= 227 * 1024 && PdLayout<128, 2>::kSmem <= 227 * 1024, "fits a CTA's shared memory");
+
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(w)));
+    return h;
+}
+__device__ __forceinline__ void cp_async8(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Arrives on `bar` once this thread's asynchronous copies so far have landed (at once if there are none).
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kPdThreads, 1)
+paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedArgs a, const uint32_t tpt) {
+    using L = PdLayout<D, NT>;
+    constexpr int kSlabs = D / 128, R = L::kRows;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float *xch = reinterpret_cast<float *>(ring + L::kRing);                  // [8 warps][8 rows][kRow]
+    float2 *scl = reinterpret_cast<float2 *>(ring + L::kRing + L::kExchange); // [stage][4 pages]
+    uint64_t *full = reinterpret_cast<uint64_t *>(scl + L::kStages * 4), *empty = full + L::kStages;
+    uint64_t *scratch = empty + L::kStages; // 40 words
+    PagedShare *share = reinterpret_cast<PagedShare *>(scratch + 40);
+    float *wm = reinterpret_cast<float *>(share + 1); // [8][R] maxima, then sums, then weights; [R] joint maximum and sum
+    float *wl = wm + 8 * 16, *ww = wl + 8 * 16, *rm = ww + 8 * 16, *rl = rm + 16, *wv = rl + 16;
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(wv + 8);
+    volatile uint32_t *never_set = abort_flag + 1;
+    volatile uint32_t *arrived = abort_flag + 2;
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < L::kStages; s++) mbar_init(&full[s], 33), mbar_init(&empty[s], 4);
+        *abort_flag = 0, *never_set = 0;
+        mbar_fence_init();
+    }
+    pdl_wait();
+    paged_share<kPdTile>(a, tpt, kPdThreads, 1, scratch, share);
+    const PagedShare sh = *share;
+    if (sh.x0 >= sh.x1) return;
+    auto give_up = [&](uint32_t bit) {
+        atomicOr(a.words, bit);
+        *abort_flag = 1;
+    };
+    const uint32_t bt = min(a.block_tokens, uint32_t(kPdTile)); // keys of one copy
+    const uint32_t G = a.group;
+    PagedWalk<kPdTile> walk(a, sh, tpt);
+    PagedItem it;
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ producer
+        uint32_t g = 0;
+        bool ok = true;
+        while (ok && walk.next(it)) {
+            const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
+            const uint32_t keys = walk.tiles.keys(it.q, it.rtile);
+            const uint32_t per_tile = kPdTile / bt;
+            auto block_of = [&](uint32_t kt) -> int32_t { // of this lane's page of a tile; -2: none
+                const uint32_t key = kt * kPdTile + lane * bt;
+                return lane < per_tile && key < keys ? table[key / a.block_tokens] : -2;
+            };
+            int32_t next = block_of(it.kt0);
+            for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
+                const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
+                int32_t block = next;
+                if (kt + 1 < it.kt1) next = block_of(kt + 1);
+                if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); ok = false; break; }
+                const bool want = block != -2;
+                const bool good = want && uint32_t(block) < a.blocks;
+                if (want && !good) atomicOr(a.words, kStatusBadBlock);
+                const uint32_t pages = __popc(__ballot_sync(0xffffffffu, good));
+                if (lane == 0) mbar_expect_tx(&full[st], pages * 2 * bt * D);
+                __syncwarp();
+                if (good) {
+                    uint8_t *dst = ring + st * L::kStage + lane * bt * D;
+                    const uint32_t key = kt * kPdTile + lane * bt;
+                    const int row = int((uint32_t(block) * a.kv_heads + it.head) * a.block_tokens + (key & (a.block_tokens - 1)));
+                    tma_load_3d(dst, &map_k, &full[st], 0, row, 0);
+                    tma_load_3d(dst + L::kSide, &map_v, &full[st], 0, row, 0);
+                }
+                if (want) // a bad block's keys are marked by its scales
+                    cp_async8(&scl[st * 4 + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
+                                                        : reinterpret_cast<const float *>(a.words + kPagedBadScale));
+                cp_async_arrive(&full[st]);
+            }
+        }
+        // let what was issued land before the shared memory goes
+        const uint32_t from = g > L::kStages ? g - L::kStages : 0;
+        for (uint32_t k = from; k < g; k++) mbar_wait(&full[k % L::kStages], (k / L::kStages) & 1, never_set, 200000u);
+        return;
+    }
+
+    // ------------------------------------------------------------ consumers
+    const uint32_t gi = lane >> 2, t = lane & 3, sub = warp & 3, team = warp >> 2;
+    uint32_t g = 0;
+    bool ok = true;
+    while (walk.next(it)) {
+        // the item's query rows as B fragments, binary16 after a power of two that brings the row's largest to [128, 256)
+        uint32_t qf[NT][D / 16][2];
+        float rs[NT][2]; // of rows 2 t and 2 t + 1: that power undone, times the softmax scale in log2 units
+        int32_t lim[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint32_t idx = nt * 8 + gi, tok = idx / G, hd = it.head * G + idx % G;
+            const bool live = tok < it.ntok && idx < tpt * G;
+            float x[kSlabs * 4][8];
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < kSlabs * 4; c++) {
+                // chunk 2 t + j of a slab, its two halves
+                const uint32_t d = (c >> 2) * 128 + (2 * t + ((c >> 1) & 1)) * 16 + (c & 1) * 8;
+                if (live) paged_load_q8(a, size_t(it.q.row0 + it.tok0 + tok) * a.q_stride + size_t(hd) * D + d, x[c]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (!live) x[c][e] = 0.f;
+                    top = fmaxf(top, fabsf(x[c][e]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = min(max(int(__float_as_uint(top) >> 23), 8), 247) - 134; // 2^(e + 7) <= top < 2^(e + 8)
+            const float up = __uint_as_float(uint32_t(127 - e) << 23);
+#pragma unroll
+            for (int c = 0; c < kSlabs * 4; c++) {
+                // a quarter chunk (4 dims) for each product: dims 0, 1 its columns 2 t, dims 2, 3 its columns 2 t + 8
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int ks = (c >> 2) * 8 + ((c >> 1) & 1) * 4 + (c & 1) * 2 + h;
+                    qf[nt][ks][0] = pack_half2(x[c][4 * h] * up, x[c][4 * h + 1] * up);
+                    qf[nt][ks][1] = pack_half2(x[c][4 * h + 2] * up, x[c][4 * h + 3] * up);
+                }
+            }
+            const float undo = __uint_as_float(uint32_t(127 + e) << 23) * a.scale_log2;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                rs[nt][j] = __shfl_sync(0xffffffffu, undo, (2 * t + j) * 4);
+                lim[nt][j] = it.lim0 + int32_t((nt * 8 + 2 * t + j) / G);
+            }
+        }
+        float o[NT][kSlabs * 8][4];
+        float m[NT][2], l[NT][2], vref = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSlabs * 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[nt][i][e] = 0.f;
+        }
+        const int32_t vis = min(int32_t(it.q.kv), it.lim0 + int32_t(it.ntok) - 1); // keys that the tile's last token sees
+        for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
+            if ((g & 1) != team) continue;
+            const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
+            if (ok && !mbar_wait(&full[st], ph, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
+            if (!ok) continue;
+            const int32_t key0 = int32_t(kt * kPdTile + sub * 16);
+            const uint32_t page = sub * 16 / bt, in = sub * 16 % bt;
+            const float2 sc = scl[st * 4 + page];
+            if (key0 < vis && sc.x >= 0.f) {
+                const uint32_t kbase = smem_u32(ring) + st * L::kStage + page * bt * D;
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+                for (int sl = 0; sl < kSlabs; sl++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t row = in + gi, at = kbase + sl * bt * 128 + row * 128 + (((2 * t + j) ^ (row & 7)) << 4);
+                        const uint4 lo = lds128(at), hi = lds128(at + 8 * 128); // key gi, key gi + 8 (the same swizzle)
+                        const uint32_t wl4[4] = {lo.x, lo.y, lo.z, lo.w}, wh4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t a0 = e4m3x2_to_h2(wl4[e]), a1 = e4m3x2_to_h2(wh4[e]);
+                            const uint32_t a2 = e4m3x2_to_h2(wl4[e] >> 16), a3 = e4m3x2_to_h2(wh4[e] >> 16);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma_f16(s[nt], a0, a1, a2, a3, qf[nt][sl * 8 + j * 4 + e][0], qf[nt][sl * 8 + j * 4 + e][1]);
+                        }
+                    }
+                const bool edge = key0 + 16 > it.lim0;
+                const float vnew = fmaxf(vref, sc.y);
+                uint32_t pb[NT][2];
+                bool need = vnew != vref;
+                float f[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float c = sc.x * rs[nt][j];
+                        s[nt][j] *= c, s[nt][2 + j] *= c;
+                        if (edge) {
+                            if (key0 + int32_t(gi) >= lim[nt][j]) s[nt][j] = -INFINITY;
+                            if (key0 + int32_t(gi) + 8 >= lim[nt][j]) s[nt][2 + j] = -INFINITY;
+                        }
+                        float mx = fmaxf(s[nt][j], s[nt][2 + j]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        f[nt][j] = 1.f;
+                        if (mx > m[nt][j] + kPdRescale) {
+                            f[nt][j] = ex2_approx(m[nt][j] - mx); // 0 for the first
+                            m[nt][j] = mx;
+                            l[nt][j] *= f[nt][j];
+                            need = true;
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, need)) {
+                    const float fv = vnew > 0.f ? vref / vnew : 1.f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int i = 0; i < kSlabs * 8; i++) {
+                            o[nt][i][0] *= f[nt][0] * fv, o[nt][i][1] *= f[nt][1] * fv;
+                            o[nt][i][2] *= f[nt][0] * fv, o[nt][i][3] *= f[nt][1] * fv;
+                        }
+                    vref = vnew;
+                }
+                const float vr = vref > 0.f ? sc.y / vref : 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float p[4];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+                        p[j] = ex2_approx(s[nt][j] - mu), p[2 + j] = ex2_approx(s[nt][2 + j] - mu);
+                        l[nt][j] += p[j] + p[2 + j];
+                    }
+                    pb[nt][0] = movmatrix_trans(pack_half2(p[0] * vr, p[1] * vr));
+                    pb[nt][1] = movmatrix_trans(pack_half2(p[2] * vr, p[3] * vr));
+                }
+                const bool tail = key0 + 16 > vis; // what lies behind the last key is any byte, NaN too: no product may read it
+#pragma unroll
+                for (int sl = 0; sl < kSlabs; sl++) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t key = 2 * t + (k & 1) + (k >> 1) * 8, row = in + key;
+                        v[k] = lds128(kbase + L::kSide + sl * bt * 128 + row * 128 + ((gi ^ (row & 7)) << 4));
+                        if (tail && key0 + int32_t(key) >= vis) v[k] = make_uint4(0, 0, 0, 0);
+                    }
+                    const uint32_t w[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                              {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t x = prmt(w[0][e], w[1][e], h ? 0x7362 : 0x5140), y = prmt(w[2][e], w[3][e], h ? 0x7362 : 0x5140);
+                            const uint32_t a0 = e4m3x2_to_h2(x), a1 = e4m3x2_to_h2(x >> 16), a2 = e4m3x2_to_h2(y), a3 = e4m3x2_to_h2(y >> 16);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][sl * 8 + e * 2 + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+
+        // ---- the eight warps' results become one: weights first, then 128 dims of 8 rows at a time
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = l[nt][j];
+                x += __shfl_xor_sync(0xffffffffu, x, 4), x += __shfl_xor_sync(0xffffffffu, x, 8), x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (gi == 0) wm[warp * R + nt * 8 + 2 * t + j] = m[nt][j], wl[warp * R + nt * 8 + 2 * t + j] = x;
+            }
+        if (lane == 0) wv[warp] = vref;
+        consumers_sync();
+        if (tid < 8 * R) {
+            const uint32_t w = tid / R, row = tid % R;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, wm[k * R + row]);
+            const float mu = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum += wl[k * R + row] * ex2_approx(wm[k * R + row] - mu);
+            ww[w * R + row] = ex2_approx(wm[w * R + row] - mu) * wv[w];
+            if (w == 0) rm[row] = top, rl[row] = sum;
+        }
+        const bool whole = it.kt0 == 0 && it.kt1 == it.tiles;
+        float *part = a.parts + (size_t(blockIdx.x) * 2 + (it.kt0 == 0 ? 1 : 0)) * a.part_floats;
+        auto finish = [&](uint32_t row, uint32_t d, float4 v, float sum) { // one row's dims d .. d + 3, unnormalised
+            const uint32_t tok = row / G, hd = it.head * G + row % G;
+            if (tok >= it.ntok || row >= tpt * G) return;
+            const size_t at = size_t(it.q.row0 + it.tok0 + tok) * a.heads + hd;
+            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); // no key: 0; NaN stays
+            v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+            if (a.q_and_gate) {
+                const float4 gt = *reinterpret_cast<const float4 *>(a.q_and_gate + at * 2 * D + D + d);
+                v.x *= sigmoid(gt.x), v.y *= sigmoid(gt.y), v.z *= sigmoid(gt.z), v.w *= sigmoid(gt.w);
+            }
+            paged_store4(a, at * D + d, v.x, v.y, v.z, v.w);
+        };
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int sl = 0; sl < kSlabs; sl++) {
+                if (nt || sl) consumers_sync(); // the exchange buffer has been read
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        // dims gi * 16 + 4 q .. + 3 of row 2 t + j; starting at q = gi keeps the lanes on different banks
+                        const uint32_t q4 = (c + gi) & 3;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (q4 == uint32_t(k)) v = make_float4(o[nt][sl * 8 + 2 * k][j], o[nt][sl * 8 + 2 * k][2 + j], o[nt][sl * 8 + 2 * k + 1][j], o[nt][sl * 8 + 2 * k + 1][2 + j]);
+                        *reinterpret_cast<float4 *>(xch + (warp * 8 + 2 * t + j) * L::kRow + gi * 16 + q4 * 4) = v;
+                    }
+                consumers_sync();
+                const uint32_t row = nt * 8 + warp, d = lane * 4;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < 8; w++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(xch + (w * 8 + warp) * L::kRow + d);
+                    const float wt = ww[w * R + row];
+                    // a warp that saw no key has weight 0 and accumulators 0
+                    v.x = fmaf(x.x, wt, v.x), v.y = fmaf(x.y, wt, v.y), v.z = fmaf(x.z, wt, v.z), v.w = fmaf(x.w, wt, v.w);
+                }
+                if (whole) finish(row, sl * 128 + d, v, rl[row]);
+                else *reinterpret_cast<float4 *>(part + row * D + sl * 128 + d) = v;
+            }
+        if (!whole) {
+            float *ml = part + R * D;
+            if (tid < R) ml[tid * 2] = rm[tid], ml[tid * 2 + 1] = rl[tid];
+            // the last CTA of the item to arrive joins the parts, in the order of the CTAs
+            const uint32_t c0 = paged_cta_of(sh, it.first), c1 = paged_cta_of(sh, it.first + it.tiles - 1), parts = c1 - c0 + 1;
+            uint32_t *counter = a.words + kPagedCounters + c0;
+            __threadfence();
+            consumers_sync();
+            if (tid == 0) {
+                const uint32_t n = atomicAdd(counter, 1);
+                if (n + 1 == parts) *counter = 0;
+                *arrived = n + 1;
+            }
+            consumers_sync();
+            if (*arrived == parts) {
+                __threadfence();
+                auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
+                float *wgt = xch; // [parts][R]
+                if (tid < R) {
+                    float top = -INFINITY, sum = 0.f;
+                    for (uint32_t p = 0; p < parts; p++) top = fmaxf(top, __ldcg(part_of(p) + R * D + tid * 2));
+                    const float mu = top == -INFINITY ? 0.f : top;
+                    for (uint32_t p = 0; p < parts; p++) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(part_of(p) + R * D + tid * 2));
+                        const float w = ex2_approx(x.x - mu);
+                        wgt[p * R + tid] = w;
+                        sum += x.y * w;
+                    }
+                    rl[tid] = sum;
+                }
+                consumers_sync();
+                for (uint32_t i = tid; i < R * D / 4; i += 256) {
+                    const uint32_t row = i * 4 / D, d = i * 4 % D;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (uint32_t p = 0; p < parts; p++) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(p) + row * D + d));
+                        const float wt = wgt[p * R + row];
+                        v.x = fmaf(x.x, wt, v.x), v.y = fmaf(x.y, wt, v.y), v.z = fmaf(x.z, wt, v.z), v.w = fmaf(x.w, wt, v.w);
+                    }
+                    finish(row, d, v, rl[row]);
+                }
+            }
+        }
+        consumers_sync(); // statistics and exchange buffer are free for the next item
+    }
+}
+
+// Keys or values as [slab of 128 dims][token rows][128 bytes]: a copy brings both slabs of `box_rows` rows.
+static int paged_map(CUtensorMap *map, const void *base, const saetta_paged_cache *c, uint32_t box_rows, uint32_t box_slabs) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(SAETTA_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available");
+    const cuuint64_t rows = cuuint64_t(c->blocks) * c->kv_heads * c->block_tokens;
+    const cuuint64_t dims[3] = {128, rows, cuuint64_t(c->head_dim / 128)};
+    const cuuint64_t strides[2] = {cuuint64_t(c->head_dim), 128};
+    const cuuint32_t box[3] = {128, box_rows, box_slabs}, el[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(SAETTA_ERR_CUDA, "paged attention: tensor map for the cache rejected");
+    return SAETTA_OK;
+}
+
+template <int D, int NT>
+static int decode_configure() {
+    SAETTA_CUDA(cudaFuncSetAttribute(paged_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PdLayout<D, NT>::kSmem));
+    return SAETTA_OK;
+}
+
+int paged_decode_configure(int) {
+    int rc = decode_configure<128, 1>();
+    if (!rc) rc = decode_configure<128, 2>();
+    if (!rc) rc = decode_configure<256, 1>();
+    if (!rc) rc = decode_configure<256, 2>();
+    return rc;
+}
+
+int launch_paged_decode(const PagedArgs &a, const saetta_paged_cache *cache, int ctas, cudaStream_t stream) {
+    CUtensorMap mk, mv;
+    const uint32_t box = std::min<uint32_t>(a.block_tokens, kPdTile), slabs = uint32_t(cache->head_dim / 128);
+    if (int rc = paged_map(&mk, cache->keys, cache, box, slabs)) return rc;
+    if (int rc = paged_map(&mv, cache->values, cache, box, slabs)) return rc;
+    const bool two = a.group > 8;
+    const uint32_t tpt = (two ? 16 : 8) / a.group; // tokens whose heads fill the product's columns
+    void (*kernel)(CUtensorMap, CUtensorMap, PagedArgs, uint32_t) = nullptr;
+    size_t smem = 0;
+    if (cache->head_dim == 256) {
+        kernel = two ? paged_decode_kernel<256, 2> : paged_decode_kernel<256, 1>;
+        smem = two ? PdLayout<256, 2>::kSmem : PdLayout<256, 1>::kSmem;
+    } else {
+        kernel = two ? paged_decode_kernel<128, 2> : paged_decode_kernel<128, 1>;
+        smem = two ? PdLayout<128, 2>::kSmem : PdLayout<128, 1>::kSmem;
+    }
+    SAETTA_CUDA(launch_pdl(kernel, dim3(unsigned(ctas)), dim3(kPdThreads), smem, stream, mk, mv, a, tpt));
+    return SAETTA_OK;
+}
+
+} // namespace saetta

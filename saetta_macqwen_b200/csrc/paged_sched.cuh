@@ -1,0 +1,229 @@
+// How an attention launch over the paged cache divides its work: the tiles of all (sequence, kv head, row tile) items,
+// one after the other, are cut into equal shares, a share for each CTA, on the device from the lengths there (so a
+// captured launch serves every length).  An item that a cut crosses leaves partials; the last CTA of it to arrive joins them.
+#pragma once
+
+#include "paged.hpp"
+
+namespace saetta {
+
+// sum over i < n of floor((a i + b) / m): counts lattice points under the line, exchanging slope and modulus as Euclid's
+// algorithm does.
+__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    uint64_t sum = 0;
+    while (true) {
+        if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
+        if (b >= m) sum += n * (b / m), b %= m;
+        const uint64_t top = a * n + b;
+        if (top < m) return sum;
+        n = top / m, b = top % m;
+        const uint64_t t = m;
+        m = a, a = t;
+    }
+}
+
+// A sequence as the kernels read it: its rows [row0, row0 + n) of q, its keys [0, kv).
+struct PagedSeq {
+    uint32_t row0, n, kv;
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, uint32_t s) {
+    PagedSeq q;
+    const uint32_t lo = min(a.row_starts[s], a.rows), hi = min(a.row_starts[s + 1], a.rows);
+    q.row0 = lo, q.n = hi > lo ? hi - lo : 0;
+    q.kv = min(a.kv_lens[s], a.table_stride * a.block_tokens);
+    return q;
+}
+
+// Key tiles (of T keys) of a sequence's row tiles (of `tpt` tokens): tile r needs the keys its last token sees.
+template <int T>
+struct PagedTiles {
+    uint32_t tpt;
+    __device__ __forceinline__ uint32_t row_tiles(const PagedSeq &q) const { return (q.n + tpt - 1) / tpt; }
+    __device__ __forceinline__ uint32_t keys(const PagedSeq &q, uint32_t r) const {
+        // more rows than keys: the first rows see nothing; every tile is given all keys
+        return q.kv < q.n ? q.kv : min(q.kv, q.kv - q.n + (r + 1) * tpt);
+    }
+    // at least one tile, so that rows that see no key are written too
+    __device__ __forceinline__ uint32_t count(const PagedSeq &q, uint32_t r) const { return max(1u, (keys(q, r) + T - 1) / T); }
+    __device__ __forceinline__ uint64_t before(const PagedSeq &q, uint32_t r) const { // of row tiles 0 .. r - 1
+        if (!r) return 0;
+        if (q.kv < q.n) return uint64_t(r) * count(q, 0);
+        const uint32_t full = r == row_tiles(q) ? r - 1 : r;
+        uint64_t sum = full ? floor_sum(full, T, tpt, q.kv - q.n + tpt + T - 1) : 0;
+        if (full != r) sum += count(q, r - 1);
+        return sum;
+    }
+    __device__ __forceinline__ uint64_t per_head(const PagedSeq &q) const { return before(q, row_tiles(q)); }
+};
+
+// One CTA's part of one item.
+struct PagedItem {
+    uint32_t seq, head, rtile;  // which item
+    PagedSeq q;
+    uint32_t tok0, ntok;        // tokens of the row tile, in the sequence
+    int32_t lim0;               // keys the tile's first token sees (<= 0: none)
+    uint32_t tiles, kt0, kt1;   // key tiles of the item, and this CTA's [kt0, kt1)
+    uint64_t first;             // flat index of the item's tile 0
+};
+
+struct PagedShare {
+    uint64_t total, x0, x1; // tiles of the launch, this CTA's
+    uint64_t head_base;     // flat index of (seq, head 0, row tile 0)
+    uint32_t ctas;          // that have a share
+    uint32_t seq, head, rtile;
+};
+
+// Walks the items of a share; every role of a CTA walks the same ones.
+template <int T>
+struct PagedWalk {
+    const PagedArgs &a;
+    PagedTiles<T> tiles;
+    uint64_t x, x1;
+    uint32_t seq, head, rtile, rtiles;
+    PagedSeq q;
+    uint32_t kt0;
+
+    __device__ __forceinline__ PagedWalk(const PagedArgs &args, const PagedShare &s, uint32_t tpt) : a(args), tiles{tpt} {
+        x = s.x0, x1 = s.x1, seq = s.seq, head = s.head, rtile = s.rtile, kt0 = 0, rtiles = 0;
+        if (x < x1) {
+            q = paged_seq(a, seq);
+            rtiles = tiles.row_tiles(q);
+            kt0 = uint32_t(x - (s.head_base + uint64_t(head) * tiles.per_head(q) + tiles.before(q, rtile)));
+        }
+    }
+    __device__ __forceinline__ bool next(PagedItem &it) {
+        if (x >= x1) return false;
+        it.seq = seq, it.head = head, it.rtile = rtile, it.q = q;
+        it.tok0 = rtile * tiles.tpt, it.ntok = min(tiles.tpt, q.n - it.tok0);
+        it.lim0 = int32_t(q.kv) - int32_t(q.n) + int32_t(it.tok0) + 1;
+        it.tiles = tiles.count(q, rtile);
+        it.kt0 = kt0;
+        it.kt1 = uint32_t(min(uint64_t(it.tiles), kt0 + (x1 - x)));
+        it.first = x - kt0;
+        x += it.kt1 - it.kt0;
+        kt0 = 0;
+        if (++rtile == rtiles) {
+            rtile = 0;
+            if (++head == a.kv_heads) {
+                head = 0;
+                if (x < x1)
+                    do q = paged_seq(a, ++seq);
+                    while (!q.n);
+                rtiles = tiles.row_tiles(q);
+            }
+        }
+        return true;
+    }
+};
+
+// The CTA whose share holds tile x.
+__device__ __forceinline__ uint32_t paged_cta_of(const PagedShare &s, uint64_t x) {
+    uint64_t c = x * s.ctas / s.total;
+    while (s.total * (c + 1) / s.ctas <= x) c++;
+    while (s.total * c / s.ctas > x) c--;
+    return uint32_t(c);
+}
+
+// Finds this CTA's share.  All `threads` threads of the block call it; `scratch` (40 words of 8 bytes) and `share` are shared memory.
+template <int T>
+__device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, uint32_t threads, uint32_t min_tiles, uint64_t *scratch, PagedShare *share) {
+    const PagedTiles<T> tiles{tpt};
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
+    uint64_t total = 0, x0 = 0;
+    for (int pass = 0; pass < 2; pass++) { // the sum first, then who holds x0
+        uint64_t carry = 0;
+        for (uint32_t base = 0; base < a.seqs; base += threads) {
+            const uint32_t s = base + tid;
+            uint64_t cost = 0;
+            if (s < a.seqs) {
+                const PagedSeq q = paged_seq(a, s);
+                if (q.n) cost = a.kv_heads * tiles.per_head(q);
+            }
+            uint64_t v = cost;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint64_t y = __shfl_up_sync(0xffffffffu, v, d);
+                if (lane >= uint32_t(d)) v += y;
+            }
+            if (lane == 31) scratch[warp] = v;
+            __syncthreads();
+            uint64_t before = carry, all = 0;
+            for (uint32_t w = 0; w < warps; w++) {
+                if (w < warp) before += scratch[w];
+                all += scratch[w];
+            }
+            v += before; // inclusive
+            if (pass == 1 && cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost;
+            if (pass == 0 && a.seqs <= threads) { // one chunk: the sums at hand serve both passes
+                total = carry + all;
+                const uint64_t ctas = min(uint64_t(gridDim.x), max(uint64_t(1), (total + min_tiles - 1) / min_tiles));
+                x0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+                if (cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost;
+            }
+            carry += all;
+            __syncthreads();
+        }
+        total = carry;
+        const uint64_t ctas = min(uint64_t(gridDim.x), max(uint64_t(1), (total + min_tiles - 1) / min_tiles));
+        x0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+        if (tid == 0) {
+            share->total = total, share->ctas = uint32_t(ctas), share->x0 = x0;
+            share->x1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+        }
+        if (a.seqs <= threads) break;
+    }
+    __syncthreads();
+    if (warp == 0 && x0 < total) {
+        const PagedSeq q = paged_seq(a, share->seq);
+        const uint64_t per = tiles.per_head(q);
+        const uint32_t head = uint32_t((x0 - share->head_base) / per);
+        const uint64_t rest = x0 - share->head_base - uint64_t(head) * per;
+        uint32_t lo = 0, hi = tiles.row_tiles(q); // the last r with before(r) <= rest, 32 candidates at a time
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo + 31) / 32, r = lo + lane * step;
+            const uint32_t le = __ballot_sync(0xffffffffu, r < hi && tiles.before(q, r) <= rest);
+            lo += (__popc(le) - 1) * step;
+            hi = min(hi, lo + step);
+        }
+        if (lane == 0) share->head = head, share->rtile = lo;
+    }
+    __syncthreads();
+}
+
+// Four values of an output row.
+__device__ __forceinline__ void paged_store4(const PagedArgs &a, size_t i, float x, float y, float z, float w) {
+    if (a.out_dtype == SAETTA_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + i) = make_float4(x, y, z, w);
+    } else if (a.out_dtype == SAETTA_F16) {
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + i) = make_uint2(pack_half2(x, y), pack_half2(z, w));
+    } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x, y), r = __floats2bfloat162_rn(z, w);
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&p), *reinterpret_cast<const uint32_t *>(&r));
+    }
+}
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+
+// 8 consecutive values of q.
+__device__ __forceinline__ void paged_load_q8(const PagedArgs &a, size_t i, float (&x)[8]) {
+    if (a.q_dtype == SAETTA_F32) {
+        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + i);
+        const float4 u = p[0], v = p[1];
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + i);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (a.q_dtype == SAETTA_BF16) {
+                x[2 * j] = __uint_as_float(u[j] << 16), x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+            } else {
+                const float2 f = h2f2(u[j]);
+                x[2 * j] = f.x, x[2 * j + 1] = f.y;
+            }
+        }
+    }
+}
+
+} // namespace saetta
