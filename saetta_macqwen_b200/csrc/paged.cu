@@ -480,6 +480,7 @@ int saetta_paged_attention_create(int device, size_t heads, size_t kv_heads, siz
     DeviceGuard guard(device);
     if (!guard.ok) return fail(SAETTA_ERR_CUDA, "PagedAttention: cannot select the device");
     if (int rc = paged_decode_configure(device)) return rc;
+    if (int rc = paged_prefill_configure(device)) return rc;
     auto *op = new (std::nothrow) saetta_paged_attention();
     if (!op) return fail(SAETTA_ERR_NO_MEM, "PagedAttention: host allocation");
     op->device = device, op->heads = heads, op->kv_heads = kv_heads, op->head_dim = head_dim;
@@ -536,7 +537,9 @@ int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *ca
     a.block_tokens = uint32_t(cache->block_tokens);
     a.q_dtype = q_dtype, a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
-    return launch_paged_decode(a, cache, op->ctas, cudaStream_t(stream));
+    // which kernel: see kPagedFewRows
+    if (batch.max_rows * a.group <= kPagedFewRows) return launch_paged_decode(a, cache, op->ctas, cudaStream_t(stream));
+    return launch_paged_prefill(a, cache, op->ctas, cudaStream_t(stream));
 }
 
 } // extern "C"

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "paged.hpp"
+#include "umma.cuh"
 
 namespace saetta {
 
@@ -224,6 +225,22 @@ __device__ __forceinline__ void paged_load_q8(const PagedArgs &a, size_t i, floa
             }
         }
     }
+}
+
+// ----------------------------------------------------------------- host side
+
+// Keys or values as [slab of 128 dims][token rows][128 bytes]: a copy brings `box_slabs` slabs of `box_rows` rows.
+inline int paged_map(CUtensorMap *map, const void *base, const saetta_paged_cache *c, uint32_t box_rows, uint32_t box_slabs) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(SAETTA_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available");
+    const cuuint64_t rows = cuuint64_t(c->blocks) * c->kv_heads * c->block_tokens;
+    const cuuint64_t dims[3] = {128, rows, cuuint64_t(c->head_dim / 128)};
+    const cuuint64_t strides[2] = {cuuint64_t(c->head_dim), 128};
+    const cuuint32_t box[3] = {128, box_rows, box_slabs}, el[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(SAETTA_ERR_CUDA, "paged attention: tensor map for the cache rejected");
+    return SAETTA_OK;
 }
 
 } // namespace saetta

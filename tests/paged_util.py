@@ -86,13 +86,16 @@ def ref_assign(lens, new, finished, free, count, tables, block, rows_cap):
 
 
 def ref_attend(q, keys, values, scales, tables, starts, kv_lens, block, scale, gate=None):
-    """q f64 [rows][heads][dim]; codes, scales as in ref_store.  Returns (out, weight of |v|, largest sum of |q k|, largest |s|),
-    the last three per (row, head): what the error bounds of the kernels go by."""
+    """q f64 [rows][heads][dim]; codes, scales as in ref_store.  Returns (out, bounds): `bounds` holds, per
+    (row, head), what the error bounds of the kernels go by: absv (the average of |v| under the weights), mag (the largest scale * sum of
+    |q k|), top (the largest |s|), wide (largest weight times value scale, times the sum of |code|), qwide (largest |q| times the largest
+    scale * sum of |k|)."""
     rows, heads, dim = q.shape
     kv_heads = keys.shape[1]
     G = heads // kv_heads
     out, absv = np.zeros((rows, heads, dim)), np.zeros((rows, heads, dim))
-    mag, top = np.zeros((rows, heads)), np.zeros((rows, heads))
+    mag, top, qwide, wide = (np.zeros((rows, heads)) for _ in range(4))
+    wide = np.zeros((rows, heads, dim))
     for s in range(len(kv_lens)):
         lo, hi, kv = starts[s], starts[s + 1], kv_lens[s]
         n = hi - lo
@@ -113,8 +116,12 @@ def ref_attend(q, keys, values, scales, tables, starts, kv_lens, block, scale, g
             p = p / np.where(t > 0, t, 1.0)
             out[lo:hi, h * G:(h + 1) * G] = np.einsum("ngk,kd->ngd", p, v)
             absv[lo:hi, h * G:(h + 1) * G] = np.einsum("ngk,kd->ngd", p, np.abs(v))
-            mag[lo:hi, h * G:(h + 1) * G], top[lo:hi, h * G:(h + 1) * G] = a.max(-1), aw.max(-1)
+            at = (slice(lo, hi), slice(h * G, (h + 1) * G))
+            mag[at], top[at] = a.max(-1), aw.max(-1)
+            qwide[at] = np.abs(qs).max(-1) * scale * np.abs(k).sum(-1).max()
+            vs = np.repeat(scales[pages, h, 1], block)[:kv]
+            wide[at] = (p * vs).max(-1)[..., None] * np.einsum("ngk,kd->ngd", ~hidden[:, None] & np.ones((1, G, 1), bool), np.abs(v / vs[:, None]))
     if gate is not None:
         g = 1.0 / (1.0 + np.exp(-gate))
-        out, absv = out * g, absv * g
-    return out, absv, mag, top
+        out, absv, wide = out * g, absv * g, wide * g
+    return out, dict(absv=absv, mag=mag, top=top, wide=wide, qwide=qwide)
