@@ -485,7 +485,7 @@ int saetta_paged_attention_create(int device, size_t heads, size_t kv_heads, siz
     if (!op) return fail(SAETTA_ERR_NO_MEM, "PagedAttention: host allocation");
     op->device = device, op->heads = heads, op->kv_heads = kv_heads, op->head_dim = head_dim;
     op->ctas = sm_count(device);
-    op->part_floats = 128 * (head_dim + 2); // 128 rows: the largest tile
+    op->part_floats = 128 * (head_dim + 2) + 4; // 128 rows: the largest tile; (m, l) of each; the value scale O is kept by
     void *p = nullptr, *w = nullptr;
     const size_t words = size_t(kPagedCounters) + 2 * size_t(op->ctas);
     cudaError_t e = cudaMalloc(&p, size_t(op->ctas) * 2 * op->part_floats * sizeof(float));

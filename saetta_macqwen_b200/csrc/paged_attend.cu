@@ -87,15 +87,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     pdl_wait();
     paged_share<kPdTile>(a, tpt, kPdThreads, 1, scratch, share);
-    const PagedShare sh = *share;
-    if (sh.x0 >= sh.x1) return;
+    if (share->x0 >= share->x1) return;
     auto give_up = [&](uint32_t bit) {
         atomicOr(a.words, bit);
         *abort_flag = 1;
     };
     const uint32_t bt = min(a.block_tokens, uint32_t(kPdTile)); // keys of one copy
     const uint32_t G = a.group;
-    PagedWalk<kPdTile> walk(a, sh, tpt);
+    PagedWalk<kPdTile> walk(a, *share, tpt);
     PagedItem it;
 
     if (warp == 8) {
@@ -198,7 +197,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[nt][i][e] = 0.f;
         }
-        const int32_t vis = min(int32_t(it.q.kv), it.lim0 + int32_t(it.ntok) - 1); // keys that the tile's last token sees
+        const int32_t vis = paged_visible(it);
         for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
             if ((g & 1) != team) continue;
             const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
@@ -376,7 +375,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             float *ml = part + R * D;
             if (tid < R) ml[tid * 2] = rm[tid], ml[tid * 2 + 1] = rl[tid];
             // the last CTA of the item to arrive joins the parts, in the order of the CTAs
-            const uint32_t c0 = paged_cta_of(sh, it.first), c1 = paged_cta_of(sh, it.first + it.tiles - 1), parts = c1 - c0 + 1;
+            const uint2 span = paged_ctas_of(*share, it);
+            const uint32_t c0 = span.x, parts = span.y;
             uint32_t *counter = a.words + kPagedCounters + c0;
             __threadfence();
             consumers_sync();

@@ -1,38 +1,46 @@
 // Attention of many rows (prompts) over the paged e4m3 cache, on the 5th-generation tensor cores.
 //
-//   t_ij = scale (q_i . kcode_j) ks[block(j)] log2 e + log2 vs[block(j)],   w = 2^(t - max t)
-//   out_i = sum_j w_ij vcode_j / sum_j (w_ij / vs[block(j)])
+//   s_ij = scale (q_i . kcode_j) ks[block(j)] log2 e,   r_j = vs[block(j)] / vref,   w = 2^(s - max s + log2 r)
+//   out_i = vref sum_j w_ij vcode_j / sum_j (w_ij / r_j)
 //
 // The codes are the operands as they lie in memory: no conversion of K or V.  tcgen05's 8-bit products run at twice the
 // 16-bit rate, and the two left-hand operands, which are not 8-bit, are split into sums of e4m3 values: a value of 8
 // significant bits (bfloat16 q) is the sum of two (4 bits each), one of 11 (binary16 q) of three.  Two products at the 8-bit rate take
-// the time of one at the 16-bit rate, with half the shared memory for K and V.  The value scales go into the exponent
-// (the running maximum is that of t), so a block's scales cost nothing for each score but the constants of one FMA, and the sum
-// of the softmax takes them out again for each block of 16 keys.
+// the time of one at the 16-bit rate, with half the shared memory for K and V.  The value scales go into the exponent,
+// relative to the largest so far (vref, by which O is kept), so a block's scales cost nothing for each score but the constants of one FMA, and
+// the sum of the softmax takes them out again for each 16 keys.  (r is not let below 2^-40: a block of zeros, whose scale is
+// 2^-126, still counts in the sum; what the bound adds to values is below 2^-40 of the largest.)
 //
 // A tile is 128 rows: `tpt` tokens x the query heads of one kv head.  Key tiles are 128 keys.  Bound by the tensor pipe: 2 * PARTS *
-// 128 * 128 * D multiply-adds for each tile at 8192 a clock and SM.  Roles: eight softmax warps (two threads for each row, 64
-// keys each), four warps that bring a tile's Q rows, one warp each for the K/V copies, the products and the scales.
+// 128 * 128 * D multiply-adds for each tile at 8192 a clock and SM.  Roles: sixteen softmax warps in two teams that take
+// tiles by turns (two threads for each row, 64 keys each), four warps that bring a tile's Q rows, one warp each for the K/V copies, the products and the scales.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged_sched.cuh"
 #include "umma.cuh"
 
 namespace saetta {
 
-constexpr int kPpRows = 128, kPpKeys = 128, kPpThreads = 512;
-constexpr float kPpShift = 6.f;   // w is kept times 2^6: e4m3 ends at 448 = 2^8.8, and its smallest steps should lie low
-constexpr float kPpRescale = 2.f; // O follows the running maximum only past this many doublings: w stays below 2^8
-constexpr int kPpScaleRing = 4;
+constexpr int kPpRows = 128, kPpKeys = 128, kPpThreads = 768;
+constexpr int kPpWarps = 16;  // of the softmax: two teams of eight, which take the tiles by turns
+constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the values
+// e4m3 ends at 448 = 2^8.8, and its smallest steps should lie low beside the weights: w is kept times 2^5.5, by a maximum that O follows only when a
+// row's scores pass it by 3 doublings (w stays below 2^8.5); then all 32 rows of the warp are brought up to date, with half a doubling to
+// spare.  (With each row following for itself past 2 doublings, some row of a CTA did so in every other tile of a random prompt of 8192 keys,
+// and the products wait for it; now in one of ten.)
+constexpr float kPpShift = 5.5f, kPpHalf = -8.f /* see split_weights */, kPpRescale = 3.f, kPpSpare = 0.5f;
+constexpr int kPpScaleRing = 4, kPpScales = 9;
 
 template <int D, int PARTS>
 struct PpLayout {
     static constexpr int kSlabs = D / 128;
     static constexpr int kQPart = kPpRows * D;
     static constexpr int kStage = kPpKeys * D; // K or V of a tile
-    static constexpr int kStages = D == 256 ? (PARTS == 2 ? 5 : 4) : 8;
-    static constexpr int kRing = kStages * kStage;
-    static constexpr int kSmem = 1024 /* alignment */ + PARTS * kQPart + kRing + 2048 /* statistics, scales, barriers */;
+    static constexpr int kKStages = D == 256 ? (PARTS == 2 ? 3 : 2) : 4, kVStages = D == 256 ? 2 : 4;
+    static constexpr int kRing = (kKStages + kVStages) * kStage;
+    static constexpr int kSmem = PARTS * kQPart + kRing + 3072 /* statistics, scales, barriers */;
+    // O; the scores of one tile; the weights' buffers, one or two
     static constexpr int kPBufs = D == 256 && PARTS == 3 ? 1 : 2;
     static constexpr int kPCols = 32 * PARTS;
     static constexpr int kTmemO = 0, kTmemS = D, kTmemP = D + 128;
@@ -40,27 +48,66 @@ struct PpLayout {
     static_assert(kSmem <= 227 * 1024, "fits a CTA's shared memory");
 };
 
-__device__ __forceinline__ void tc_mma8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The products are issued by whole warps in step, one lane's predicate inside the instruction, from operands that are the same in every
+// lane as far as the compiler can tell (uniform()): under a branch of one lane it takes 120 clocks to bring the operands of each product to
+// the registers that the instruction reads, and the pipe needs 64 for the product.
+// Descriptors come as their low words; the high word, the same for all (stride 1024 bytes, 128-byte swizzle), is an immediate.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void tc_mma8(uint32_t leader, uint32_t d_tmem, uint32_t adesc, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(adesc), "r"(bdesc), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
         : "memory");
 }
 // A from tensor memory: row m in lane m, four e4m3 values in a column.
-__device__ __forceinline__ void tc_mma8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma8_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], b, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(bdesc), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-        : "memory");
+__device__ __forceinline__ void tc_commit_if(uint32_t leader, uint64_t *bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(smem_u32(bar)), "r"(leader)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3ffffu) >> 4) | (lbo_bytes >> 4) << 16; }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
+// Scores from the `see`-th on belong to keys that the row does not see.
+__device__ __forceinline__ void mask32(uint32_t (&s)[32], int32_t see) {
+    if (see < 32) {
+#pragma unroll
+        for (int k = 0; k < 32; k++)
+            if (k >= see) s[k] = 0xff800000u; // -infinity
+    }
+}
+// Two FMAs, two additions, in one instruction each; the largest of three.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ uint32_t f2_to_e4m3x2(float lo, float hi) {
     uint16_t d;
@@ -77,71 +124,137 @@ __device__ __forceinline__ uint32_t e4m3x2_as_h2(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(w)));
     return h;
 }
-// Four values as sums of PARTS e4m3 values each: word p holds the four p-th terms.  Every remainder is exact (a value less its
+// N values as sums of PARTS e4m3 values each: w[p] holds the p-th terms, four to a word.  Every remainder is exact (a value less its
 // rounding to fewer bits), so the sum is off by the last term's rounding alone: 2^-8 of the value with two, 2^-12 with three,
-// and 2^-10 of a unit below e4m3's normal range.
-template <int PARTS>
-__device__ __forceinline__ void split4(float a, float b, float c, float d, uint32_t (&w)[PARTS]) {
+// and 2^-10 of a unit below e4m3's normal range.  Stage by stage over all values: each step has the latency of a conversion.
+template <int PARTS, int N>
+__device__ __forceinline__ void split(float (&x)[N], uint32_t (&w)[PARTS][N / 4]) {
+    uint32_t t[N / 2];
     if constexpr (PARTS == 2) {
         // by way of binary16, whose 11 bits hold the two terms
-        const uint32_t h0 = pack_half2(a, b), h1 = pack_half2(c, d);
-        const uint32_t t0 = h2_to_e4m3x2(h0), t1 = h2_to_e4m3x2(h1);
-        w[0] = t0 | t1 << 16;
-        w[1] = h2_to_e4m3x2(hsub2_u32(h0, e4m3x2_as_h2(t0))) | h2_to_e4m3x2(hsub2_u32(h1, e4m3x2_as_h2(t1))) << 16;
+        uint32_t h[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) h[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) t[i] = h2_to_e4m3x2(h[i]);
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) w[0][i] = prmt(t[2 * i], t[2 * i + 1], 0x5410);
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) h[i] = hsub2_u32(h[i], e4m3x2_as_h2(t[i]));
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) t[i] = h2_to_e4m3x2(h[i]);
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) w[1][i] = prmt(t[2 * i], t[2 * i + 1], 0x5410);
     } else {
 #pragma unroll
         for (int p = 0; p < PARTS; p++) {
-            const uint32_t t0 = f2_to_e4m3x2(a, b), t1 = f2_to_e4m3x2(c, d);
-            w[p] = t0 | t1 << 16;
-            const float2 f0 = h2f2(e4m3x2_as_h2(t0)), f1 = h2f2(e4m3x2_as_h2(t1));
-            a -= f0.x, b -= f0.y, c -= f1.x, d -= f1.y;
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) t[i] = f2_to_e4m3x2(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+            for (int i = 0; i < N / 4; i++) w[p][i] = prmt(t[2 * i], t[2 * i + 1], 0x5410);
+            if (p + 1 < PARTS) {
+#pragma unroll
+                for (int i = 0; i < N / 2; i++) {
+                    const float2 f = h2f2(e4m3x2_as_h2(t[i]));
+                    x[2 * i] -= f.x, x[2 * i + 1] -= f.y;
+                }
+            }
         }
     }
 }
-__device__ __forceinline__ void pair_sync(uint32_t quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+// The same for weights, which are not negative, in a third of the time: they come times 2^-8 (kPpHalf), where the exponent field of a binary16
+// value is that of its e4m3 code, subnormals included, so that the code is the value's bits 14 .. 7.  Each term but the last is cut off there,
+// what remains is exact, and the last is rounded (half up): two terms are off by 2^-8 of the weight at most, three hold the binary16 value.
+template <int PARTS>
+__device__ __forceinline__ void split_weights(const float *x, uint32_t (&w)[PARTS]) { // of four
+    uint32_t h0 = pack_half2(x[0], x[1]), h1 = pack_half2(x[2], x[3]);
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) {
+        const uint32_t r = p + 1 == PARTS ? 0x00800080u : 0u;
+        w[p] = prmt(h0 * 2 + r, h1 * 2 + r, 0x7531); // the codes stand in the upper bytes
+        if (p + 1 < PARTS) h0 = hsub2_u32(h0, h0 & 0xff80ff80u), h1 = hsub2_u32(h1, h1 & 0xff80ff80u);
+    }
+}
+// A bounded wait of a whole warp, in few instructions (there are forty of them): by polls, each of which the hardware holds for a while, up to
+// about a microsecond.  SLEEP: nanoseconds between polls, for roles that run ahead of the others.
+template <int SLEEP>
+__device__ __forceinline__ bool short_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
+    bool ok = true;
+#pragma unroll 1
+    for (uint32_t n = 0; ok && !mbar_test(bar, parity); n++) {
+        if (SLEEP) __nanosleep(SLEEP);
+        if ((n & 63) == 63) ok = n <= 4000000u && !*abort_flag;
+    }
+    return __all_sync(0xffffffffu, ok);
+}
 __device__ __forceinline__ float lg2_approx(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
+// What the roles of a CTA need of an item: one warp walks the items and leaves this in a small ring of shared memory.  (With a walk in
+// each role's registers they spilled, and of the 256 KB an SM has for L1 and shared memory this kernel leaves L1 so little that the spills
+// missed it: every step of every role took hundreds of clocks.)
+struct PpItem {
+    uint32_t kt0, kt1;      // key tiles; kt0 == kt1: no more items
+    int32_t lim0, vis;      // keys that the first and the last token see
+    uint32_t seq, head;
+    uint32_t row0, ntok;    // first row of q, tokens
+    uint32_t keys;          // to be copied
+    uint32_t c0, parts;     // the CTAs it lies in
+    uint32_t pad;
+};
+constexpr int kPpItems = 4;
+constexpr int kPpItemReaders = 2 /* products */ + 1 /* scales */ + 4 /* Q rows */ + kPpWarps;
+
 template <int D, int PARTS>
 __global__ void __launch_bounds__(kPpThreads, 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedArgs a, const uint32_t tpt) {
     using L = PpLayout<D, PARTS>;
-    constexpr int kSlabs = L::kSlabs, NST = L::kStages, NP = L::kPBufs;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int kSlabs = L::kSlabs, NK = L::kKStages, NV = L::kVStages, NP = L::kPBufs;
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sQ = smem;                                  // [part][slab][128 rows][128 dims]
-    uint8_t *ring = sQ + PARTS * L::kQPart;              // [stage][slab][128 keys][128 dims], K and V by turns
-    __nv_bfloat16 *xch = reinterpret_cast<__nv_bfloat16 *>(ring + L::kRing); // [2][2 halves][128 rows] maxima, rounded up
-    float *lx = reinterpret_cast<float *>(xch);              // at a tile's end: [2 halves][128 rows] sums
-    float4 *scl = reinterpret_cast<float4 *>(lx + 256);      // [kPpScaleRing][8]: key scale, log2 and reciprocal of the value scale, bad
-    uint64_t *bars = reinterpret_cast<uint64_t *>(scl + kPpScaleRing * 8);
-    uint64_t *full = bars, *empty = bars + 8, *sc_full = bars + 16, *sc_empty = bars + 20, *q_full = bars + 24, *q_empty = bars + 25,
-             *s_full = bars + 26, *s_free = bars + 27, *p_full = bars + 28, *pv_done = bars + 30, *o_final = bars + 32, *o_empty = bars + 33;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 34);
+    uint8_t *ring = sQ + PARTS * L::kQPart;              // [K stages, V stages][slab][128 keys][128 dims]
+    uint8_t *ring_v = ring + NK * L::kStage;
+    // the statistics' area, 3 KB
+    __nv_bfloat16 *xch = reinterpret_cast<__nv_bfloat16 *>(ring + L::kRing); // [team][half][128 rows]: maxima, rounded up
+    float *lx = reinterpret_cast<float *>(xch);                              // at a tile's end: [2][128 rows] sums
+    __nv_bfloat16 *mpub = xch + 512;                                         // [2][128 rows]: the running maxima after a tile
+    float2 *scl = reinterpret_cast<float2 *>(mpub + 256);                    // [kPpScaleRing][8]: key scale (-1: bad block), log2 r; then
+                                                                             // what vref falls by against the tile before, vref
+    PpItem *items = reinterpret_cast<PpItem *>(scl + kPpScaleRing * kPpScales);
+    PagedShare *share = reinterpret_cast<PagedShare *>(items + kPpItems);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(share + 1);
+    uint64_t *k_full = bars, *v_full = bars + 4, *k_empty = bars + 8, *v_empty = bars + 12, *sc_full = bars + 16, *sc_empty = bars + 20,
+             *item_full = bars + 24, *item_empty = bars + 28, *s_full = bars + 32 /* one for each team: a wait by parity must not find the other's phase */,
+             *p_full = bars + 34, *pv_done = bars + 36, *q_full = bars + 38, *q_empty = bars + 39, *s_free = bars + 40, *o_final = bars + 41,
+             *o_empty = bars + 42, *all_met = bars + 43, *pair_met = bars + 44 /* [team][row quarter] */, *m_full = bars + 52 /* [2][4 row quarters] */;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 60);
     volatile uint32_t *abort_flag = tmem_slot + 1, *never_set = tmem_slot + 2, *arrived = tmem_slot + 3;
-    // the share's scratch is the Q area, free until the roles begin
-    uint64_t *scratch = reinterpret_cast<uint64_t *>(sQ);
-    PagedShare *share = reinterpret_cast<PagedShare *>(scratch + 40);
-    uint8_t *row_e = reinterpret_cast<uint8_t *>(bars + 40); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
+    uint8_t *row_e = reinterpret_cast<uint8_t *>(bars + 62); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
 
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (smem_u32(smem) & 1023) { // the swizzle and the descriptors count on it
+        if (threadIdx.x == 0) atomicOr(a.words, kStatusMmaTimeout);
+        return;
+    }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NST; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        for (int s = 0; s < kPpScaleRing; s++) mbar_init(&sc_full[s], 1), mbar_init(&sc_empty[s], 9);
-        mbar_init(q_full, 4), mbar_init(q_empty, 9), mbar_init(s_full, 1), mbar_init(s_free, 8), mbar_init(o_final, 1), mbar_init(o_empty, 8);
-        for (int s = 0; s < 2; s++) mbar_init(&p_full[s], 8), mbar_init(&pv_done[s], 1);
+        for (int s = 0; s < 4; s++) {
+            mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
+            mbar_init(&sc_full[s], 1), mbar_init(&sc_empty[s], 1), mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], kPpItemReaders);
+        }
+        for (int s = 0; s < 2; s++) mbar_init(&s_full[s], 1), mbar_init(&p_full[s], kPpWarps / 2), mbar_init(&pv_done[s], 1);
+        for (int s = 0; s < 8; s++) mbar_init(&pair_met[s], 2), mbar_init(&m_full[s], 1);
+        mbar_init(q_full, 4), mbar_init(q_empty, 1 + kPpWarps), mbar_init(s_free, kPpWarps / 2), mbar_init(o_final, 1), mbar_init(o_empty, kPpWarps);
+        mbar_init(all_met, kPpWarps);
         *abort_flag = 0, *never_set = 0;
         mbar_fence_init();
     }
     pdl_wait();
-    paged_share<kPpKeys>(a, tpt, kPpThreads, 1, scratch, share);
-    const PagedShare sh = *share;
-    if (sh.x0 >= sh.x1) return; // (the whole CTA)
-    if (warp == 13) {
+    paged_share<kPpKeys>(a, tpt, kPpThreads, 1, reinterpret_cast<uint64_t *>(sQ), share); // (its scratch is the Q area, free until the roles begin)
+    if (share->x0 >= share->x1) return; // (the whole CTA)
+    if (warp == 21) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -150,159 +263,211 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + L::kTmemO, tmem_s = tmem + L::kTmemS, tmem_p = tmem + L::kTmemP;
-    auto give_up = [&](uint32_t bit) {
-        atomicOr(a.words, bit);
-        *abort_flag = 1;
-    };
-    const uint32_t G = a.group;
-    PagedWalk<kPpKeys> walk(a, sh, tpt);
-    PagedItem it;
+    // Waits are bounded: one that gives up leaves its role, sets the status and the flag that ends the others' waits.  (No role waits at a
+    // named barrier, which would have no bound.)
+#define PP_WAIT_FOR(sleep, bar, parity, bit)            \
+    if (!short_wait<sleep>(bar, parity, abort_flag)) {  \
+        atomicOr(a.words, bit);                         \
+        *abort_flag = 1;                                \
+        goto done;                                      \
+    }
+#define PP_WAIT(bar, parity, bit) PP_WAIT_FOR(0, bar, parity, bit)
+#define PP_WAIT_AHEAD(bar, parity, bit) PP_WAIT_FOR(64, bar, parity, bit)
 
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12) {
-            // ------------------------------------------------------------ K and V copies, in the order of the products: K0 K1 V0 K2 V1 ...
+    uint32_t copied_k = 0, copied_v = 0; // of the copying warp
+
+    // registers: 512 x 96 + 256 x 48 = the 768 x 80 of the launch
+    if (warp >= 20) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 20) {
+            // ------------------------------------------------------------ items; K and V copies: K0 K1 K2 V0 K3 V1 ... through all items
+            // (A K stage is free once the scores that use it are done, and those wait for no value product later than the one two
+            // tiles before them.)
             const uint32_t bt = min(a.block_tokens, uint32_t(kPpKeys)), per_tile = kPpKeys / bt;
-            uint32_t r = 0;
-            bool ok = true;
-            while (ok && walk.next(it)) {
-                const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
-                const uint32_t keys = walk.tiles.keys(it.q, it.rtile), page = lane / kSlabs, slab = lane % kSlabs;
-                auto block_of = [&](uint32_t kt) -> int32_t {
-                    const uint32_t key = kt * kPpKeys + page * bt;
-                    return page < per_tile && key < keys ? table[key / a.block_tokens] : -2;
-                };
-                auto load = [&](int32_t block, bool values) {
-                    const uint32_t st = r % NST, ph = (r / NST) & 1;
-                    if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); return false; }
-                    const bool good = block != -2 && uint32_t(block) < a.blocks;
-                    const uint32_t copies = __popc(__ballot_sync(0xffffffffu, good));
-                    if (lane == 0) mbar_expect_tx(&full[st], copies * bt * 128);
-                    __syncwarp();
-                    if (good)
-                        tma_load_3d(ring + st * L::kStage + slab * (kPpKeys * 128) + page * bt * 128, values ? &map_v : &map_k, &full[st], 0,
-                                    int((uint32_t(block) * a.kv_heads + it.head) * a.block_tokens), int(slab));
-                    r++;
-                    return true;
-                };
-                int32_t cur = block_of(it.kt0), prev = -2;
-                for (uint32_t kt = it.kt0; ok && kt < it.kt1; kt++) {
-                    const int32_t next = kt + 1 < it.kt1 ? block_of(kt + 1) : -2;
-                    ok = load(cur, false);
-                    if (ok && kt > it.kt0) ok = load(prev, true);
-                    prev = cur, cur = next;
-                }
-                if (ok) ok = load(prev, true);
-            }
-            for (uint32_t k = r > NST ? r - NST : 0; k < r; k++) mbar_wait(&full[k % NST], (k / NST) & 1, never_set, 200000u);
-        } else if (warp == 13) {
-            // ------------------------------------------------------------ products
-            constexpr uint32_t idesc_s = (1u << 4) | (uint32_t(kPpKeys >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
-            constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
-            uint32_t r = 0, g = 0, tc = 0; // ring places, tiles, items so far
-            bool ok = true;
-            while (ok && walk.next(it)) {
-                const uint32_t nb = it.kt1 - it.kt0;
-                const int32_t vis = min(int32_t(it.q.kv), it.lim0 + int32_t(it.ntok) - 1);
-                if (!mbar_wait(q_full, tc & 1, abort_flag)) { give_up(kStatusFullTimeout); break; }
-                auto values = [&](uint32_t j) { // O += P V of tile j
-                    const uint32_t st = r % NST, ph = (r / NST) & 1, gj = g + j, pb = gj % NP, ss = gj % kPpScaleRing;
-                    if (!mbar_wait(&full[st], ph, abort_flag)) { give_up(kStatusFullTimeout); return false; }
-                    if (!mbar_wait(&sc_full[ss], (gj / kPpScaleRing) & 1, abort_flag)) { give_up(kStatusFullTimeout); return false; }
-                    // rows behind the last key, and of bad blocks, may hold NaN, which a weight of 0 does not silence
-                    const int32_t key0 = int32_t((it.kt0 + j) * kPpKeys);
-                    const uint32_t bad = __ballot_sync(0xffffffffu, lane < 8 && scl[ss * 8 + lane].w != 0.f);
-                    if (key0 + kPpKeys > vis || bad) {
-                        for (uint32_t i = lane; i < kPpKeys * 8 * kSlabs; i += 32) {
-                            const uint32_t key = (i >> 3) % kPpKeys, slab = i / (kPpKeys * 8);
-                            if (key0 + int32_t(key) >= vis || (bad >> (key >> 4) & 1))
-                                *reinterpret_cast<uint4 *>(ring + st * L::kStage + slab * (kPpKeys * 128) + key * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            const uint32_t page = lane / kSlabs, slab = lane % kSlabs;
+            PagedWalk<kPpKeys> walk(a, *share, tpt);
+            const uint32_t tiles = walk.end;
+            uint32_t ni = 0, kk = 0, kk1 = 0;
+            int row[kPpAhead + 2] = {-1, -1, -1, -1}; // this lane's row of the cache for the next tile, the tile at hand, and those before; -1: none
+            const int32_t *table = nullptr;
+            uint32_t keys = 0, head = 0;
+            for (uint32_t i = 0; i < tiles + kPpAhead + 1; i++) { // the copies of a tile are issued a step after its page has been looked up
+#pragma unroll
+                for (int k = kPpAhead + 1; k > 0; k--) row[k] = row[k - 1];
+                if (i < tiles) {
+                    if (kk == kk1) {
+                        PagedItem it;
+                        walk.next(it);
+                        PP_WAIT_AHEAD(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1, kStatusEmptyTimeout);
+                        const uint2 span = paged_ctas_of(*share, it);
+                        kk = it.kt0, kk1 = it.kt1, keys = walk.tiles.keys(it.q, it.rtile), head = it.head;
+                        table = a.tables + size_t(it.seq) * a.table_stride;
+                        if (lane == 0) {
+                            items[ni % kPpItems] = PpItem{it.kt0, it.kt1, it.lim0, paged_visible(it), it.seq, it.head, it.q.row0 + it.tok0, it.ntok, keys, span.x, span.y, 0};
+                            mbar_arrive(&item_full[ni % kPpItems]);
                         }
-                        fence_async_smem();
+                        __syncwarp();
+                        ni++;
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sc_empty[ss]);
-                    if (j == 0 && !mbar_wait(o_empty, (tc & 1) ^ 1, abort_flag)) { give_up(kStatusMmaTimeout); return false; }
-                    if (!mbar_wait(&p_full[pb], (gj / NP) & 1, abort_flag)) { give_up(kStatusMmaTimeout); return false; }
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint64_t bd = umma_desc(smem_u32(ring) + st * L::kStage, kPpKeys * 128, 1024);
-#pragma unroll
-                        for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                            for (int ks = 0; ks < kPpKeys / 32; ks++)
-                                tc_mma8_ts(tmem_o, tmem_p + pb * L::kPCols + p * 32 + ks * 8, bd + uint64_t((ks * 4096) >> 4), idesc_o, j > 0 || p > 0 || ks > 0);
-                        tc_commit(&empty[st]);
-                        tc_commit(&pv_done[pb]);
-                        if (j + 1 == nb) tc_commit(o_final);
+                    const uint32_t key = kk * kPpKeys + page * bt;
+                    row[0] = -1;
+                    if (page < per_tile && key < keys) {
+                        const uint32_t block = uint32_t(table[key / a.block_tokens]);
+                        if (block < a.blocks) row[0] = int((block * a.kv_heads + head) * a.block_tokens);
                     }
-                    __syncwarp();
-                    r++;
-                    return true;
-                };
-                for (uint32_t j = 0; ok && j < nb; j++) {
-                    const uint32_t st = r % NST, ph = (r / NST) & 1, gj = g + j;
-                    if (!mbar_wait(&full[st], ph, abort_flag)) { give_up(kStatusFullTimeout); ok = false; break; }
-                    if (!mbar_wait(s_free, (gj & 1) ^ 1, abort_flag)) { give_up(kStatusMmaTimeout); ok = false; break; }
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint64_t ad = umma_desc(smem_u32(sQ), 16, 1024), bd = umma_desc(smem_u32(ring) + st * L::kStage, 16, 1024);
-#pragma unroll
-                        for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                            for (int ks = 0; ks < D / 32; ks++) {
-                                const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-                                tc_mma8(tmem_s, ad + uint64_t((p * L::kQPart + off) >> 4), bd + uint64_t(off >> 4), idesc_s, p > 0 || ks > 0);
-                            }
-                        tc_commit(&empty[st]);
-                        tc_commit(s_full);
-                        if (j + 1 == nb) tc_commit(q_empty);
-                    }
-                    __syncwarp();
-                    r++;
-                    if (j > 0) ok = values(j - 1);
+                    kk++;
                 }
-                if (ok) ok = values(nb - 1);
-                g += nb, tc++;
+                const uint32_t dst = slab * (kPpKeys * 128) + page * bt * 128;
+                if (i >= 1 && i <= tiles) {
+                    const uint32_t g = i - 1, st = g % NK, n = __popc(__ballot_sync(0xffffffffu, row[1] >= 0));
+                    PP_WAIT(&k_empty[st], (g / NK & 1) ^ 1, kStatusEmptyTimeout);
+                    if (lane == 0) mbar_expect_tx(&k_full[st], n * bt * 128);
+                    copied_k = g + 1;
+                    __syncwarp();
+                    if (row[1] >= 0) tma_load_3d(ring + st * L::kStage + dst, &map_k, &k_full[st], 0, row[1], int(slab));
+                }
+                if (i >= kPpAhead + 1) {
+                    const uint32_t g = i - kPpAhead - 1, st = g % NV, n = __popc(__ballot_sync(0xffffffffu, row[kPpAhead + 1] >= 0));
+                    PP_WAIT(&v_empty[st], (g / NV & 1) ^ 1, kStatusEmptyTimeout);
+                    if (lane == 0) mbar_expect_tx(&v_full[st], n * bt * 128);
+                    copied_v = g + 1;
+                    __syncwarp();
+                    if (row[kPpAhead + 1] >= 0) tma_load_3d(ring_v + st * L::kStage + dst, &map_v, &v_full[st], 0, row[kPpAhead + 1], int(slab));
+                }
             }
-        } else if (warp == 14) {
+            PP_WAIT_AHEAD(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1, kStatusEmptyTimeout);
+            if (lane == 0) {
+                items[ni % kPpItems].kt0 = items[ni % kPpItems].kt1 = 0;
+                mbar_arrive(&item_full[ni % kPpItems]);
+            }
+        } else if (warp == 21) {
+            // ------------------------------------------------------------ score products
+            constexpr uint32_t idesc = (1u << 4) | (uint32_t(kPpKeys >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
+            const uint32_t ad = uniform(desc_low(smem_u32(sQ), 16)), bd0 = uniform(desc_low(smem_u32(ring), 16)), ts = uniform(tmem_s);
+            const uint32_t leader = lane == 0;
+            uint32_t g = 0;
+            for (uint32_t ni = 0;; ni++) {
+                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+                const uint32_t end = g + uniform(items[ni % kPpItems].kt1 - items[ni % kPpItems].kt0);
+                if (g == end) break;
+                __syncwarp();
+                if (leader) mbar_arrive(&item_empty[ni % kPpItems]);
+                PP_WAIT(q_full, ni & 1, kStatusFullTimeout);
+                for (; g < end; g++) {
+                    const uint32_t st = g % NK;
+                    PP_WAIT(&k_full[st], g / NK & 1, kStatusFullTimeout);
+                    PP_WAIT(s_free, (g & 1) ^ 1, kStatusMmaTimeout);
+                    tc_fence_after();
+                    __syncwarp();
+                    const uint32_t bd = bd0 + st * (L::kStage >> 4);
+#pragma unroll
+                    for (uint32_t k = 0; k < PARTS * D / 32; k++) // 32 dims of one term; slabs of 128 dims lie 16 KB apart, the terms of Q behind one another
+                        tc_mma8(leader, ts, ad + (k >> 2) * 1024 + (k & 3) * 2, bd + (k >> 2) % kSlabs * 1024 + (k & 3) * 2, idesc, k);
+                    tc_commit_if(leader, &s_full[g & 1]);
+                    tc_commit_if(leader, &k_empty[st]);
+                    if (g + 1 == end) tc_commit_if(leader, q_empty);
+                }
+            }
+        } else if (warp == 22) {
             // ------------------------------------------------------------ scales of each 16 keys
             uint32_t g = 0;
-            bool ok = true;
-            while (ok && walk.next(it)) {
+            for (uint32_t ni = 0;; ni++) {
+                PP_WAIT_AHEAD(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+                const PpItem &it = items[ni % kPpItems];
+                const uint32_t keys = it.keys, head = it.head, kt1 = it.kt1;
+                uint32_t kt = it.kt0;
                 const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
-                const uint32_t keys = walk.tiles.keys(it.q, it.rtile);
-                for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
+                if (kt == kt1) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
+                float vref = 0.f;
+                for (; kt < kt1; kt++, g++) {
                     const uint32_t ss = g % kPpScaleRing, key = kt * kPpKeys + lane * 16;
-                    float4 v = make_float4(1.f, 0.f, 1.f, 0.f); // behind the last key: masked whatever stands here
+                    float2 v = make_float2(1.f, 0.f); // behind the last key: masked whatever stands here
+                    bool good = false;
                     if (lane < 8 && key < keys) {
                         const int32_t block = table[key / a.block_tokens];
                         if (uint32_t(block) < a.blocks) {
-                            const float2 s = *reinterpret_cast<const float2 *>(a.scales + (size_t(block) * a.kv_heads + it.head) * 2);
-                            v = make_float4(s.x, lg2_approx(s.y), 1.f / s.y, 0.f);
+                            const float2 s = *reinterpret_cast<const float2 *>(a.scales + (size_t(block) * a.kv_heads + head) * 2);
+                            v = make_float2(fmaxf(s.x, FLT_MIN), s.y);
+                            good = true;
                         } else {
-                            v.w = 1.f;
+                            v.x = -1.f;
                             atomicOr(a.words, kStatusBadBlock);
                         }
                     }
-                    if (!mbar_wait(&sc_empty[ss], ((g / kPpScaleRing) & 1) ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); ok = false; break; }
-                    if (lane < 8) scl[ss * 8 + lane] = v;
+                    float top = v.y;
+#pragma unroll
+                    for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    top = fmaxf(fmaxf(__shfl_sync(0xffffffffu, top, 0), FLT_MIN), vref);
+                    v.y = good ? fmaxf(lg2_approx(v.y / top), -40.f) : 0.f;
+                    if (lane == 8) v = make_float2(vref > 0.f ? vref / top : 1.f, top);
+                    vref = top;
+                    PP_WAIT_AHEAD(&sc_empty[ss], (g / kPpScaleRing & 1) ^ 1, kStatusEmptyTimeout);
+                    if (lane < kPpScales) scl[ss * kPpScales + lane] = v;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[ss]);
                 }
             }
+        } else {
+            // ------------------------------------------------------------ value products
+            constexpr uint32_t idesc = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
+            const uint32_t bd0 = uniform(desc_low(smem_u32(ring_v), kPpKeys * 128)), to = uniform(tmem_o), tp = uniform(tmem_p);
+            const uint32_t leader = lane == 0;
+            uint32_t g = 0;
+            for (uint32_t ni = 0;; ni++) {
+                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+                const int32_t vis = items[ni % kPpItems].vis;
+                const uint32_t kt0 = uniform(items[ni % kPpItems].kt0), kt1 = uniform(items[ni % kPpItems].kt1);
+                if (kt0 == kt1) break;
+                __syncwarp();
+                if (leader) mbar_arrive(&item_empty[ni % kPpItems]);
+                for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
+                    const uint32_t st = g % NV, pb = g % NP, ss = g % kPpScaleRing;
+                    PP_WAIT(&v_full[st], g / NV & 1, kStatusFullTimeout);
+                    PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1, kStatusFullTimeout);
+                    // rows behind the last key, and of bad blocks, may hold NaN, which a weight of 0 does not silence
+                    const int32_t key0 = int32_t(kt * kPpKeys);
+                    const uint32_t bad = __ballot_sync(0xffffffffu, lane < 8 && scl[ss * kPpScales + (lane & 7)].x < 0.f);
+                    if (key0 + kPpKeys > vis || bad) {
+                        for (uint32_t k = lane; k < kPpKeys * 8 * kSlabs; k += 32) {
+                            const uint32_t key = (k >> 3) % kPpKeys, slab = k / (kPpKeys * 8);
+                            if (key0 + int32_t(key) >= vis || (bad >> (key >> 4) & 1))
+                                *reinterpret_cast<uint4 *>(ring_v + st * L::kStage + slab * (kPpKeys * 128) + key * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+                    if (kt == kt0) PP_WAIT(o_empty, (ni & 1) ^ 1, kStatusMmaTimeout);
+                    PP_WAIT(&p_full[pb], g / NP & 1, kStatusMmaTimeout);
+                    tc_fence_after();
+                    __syncwarp();
+                    const uint32_t bd = bd0 + st * (L::kStage >> 4), ap = tp + pb * L::kPCols;
+#pragma unroll
+                    for (uint32_t k = 0; k < PARTS * kPpKeys / 32; k++) // 32 keys of one term
+                        tc_mma8_ts(leader, to, ap + k * 8, bd + (k & 3) * 256, idesc, (kt - kt0) | k);
+                    tc_commit_if(leader, &pv_done[g & 1]);
+                    tc_commit_if(leader, &v_empty[st]);
+                    tc_commit_if(leader, &sc_empty[ss]); // (its softmax is over too)
+                    if (kt + 1 == kt1) tc_commit_if(leader, o_final);
+                }
+            }
         }
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    } else if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         // ------------------------------------------------------------ a tile's Q rows, a thread for each
-        const uint32_t row = threadIdx.x - 256, tok = row / G, hq = row % G;
-        uint32_t tc = 0;
-        while (walk.next(it)) {
-            const bool live = tok < it.ntok && row < tpt * G;
-            const size_t at = live ? size_t(it.q.row0 + it.tok0 + tok) * a.q_stride + size_t(it.head * G + hq) * D : 0;
+        const uint32_t row = threadIdx.x - 512, tok = row / a.group, hq = row % a.group;
+        for (uint32_t ni = 0;; ni++) {
+            PP_WAIT_AHEAD(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+            const PpItem &it = items[ni % kPpItems];
+            if (it.kt0 == it.kt1) break;
+            const bool live = tok < it.ntok && row < tpt * a.group;
+            const size_t at = live ? size_t(it.row0 + tok) * a.q_stride + size_t(it.head * a.group + hq) * D : 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
             float top = 0.f;
             if (live) {
-#pragma unroll 8
+#pragma unroll 2
                 for (int c = 0; c < D; c += 8) {
                     float x[8];
                     paged_load_q8(a, at + c, x);
@@ -314,160 +479,205 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const int e = min(max(int(__float_as_uint(top) >> 23), 8), 247) - 134;
             const float up = __uint_as_float(uint32_t(127 - e) << 23);
             // the products of the tile before have read the old Q, and its softmax the old factors
-            if (!mbar_wait(q_empty, (tc & 1) ^ 1, abort_flag)) { give_up(kStatusMmaTimeout); break; }
+            PP_WAIT_AHEAD(q_empty, (ni & 1) ^ 1, kStatusMmaTimeout);
             row_e[row] = uint8_t(127 + e);
-#pragma unroll 2
+#pragma unroll 1
             for (int c = 0; c < D; c += 16) {
-                float x[2][8];
-                if (live) {
-                    paged_load_q8(a, at + c, x[0]), paged_load_q8(a, at + c + 8, x[1]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) x[0][k] = x[1][k] = 0.f;
-                }
-                uint32_t w[4][PARTS];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float *y = &x[k >> 1][(k & 1) * 4];
-                    split4<PARTS>(y[0] * up, y[1] * up, y[2] * up, y[3] * up, w[k]);
-                }
                 uint8_t *dst = sQ + (c >> 7) * (kPpRows * 128) + row * 128 + ((((c >> 4) & 7) ^ (row & 7)) << 4);
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) *reinterpret_cast<uint4 *>(dst + p * L::kQPart) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+                for (int h = 0; h < 2; h++) {
+                    float x[8];
+                    if (live) {
+                        paged_load_q8(a, at + c + 8 * h, x);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) x[k] = 0.f;
+                    }
+                    uint32_t w[PARTS][2];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] *= up;
+                    split<PARTS, 8>(x, w);
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) *reinterpret_cast<uint2 *>(dst + p * L::kQPart + 8 * h) = make_uint2(w[p][0], w[p][1]);
+                }
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
-            tc++;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
         // ------------------------------------------------------------ softmax; a tile's end
-        const uint32_t quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+        // Two teams of eight warps take the tiles by turns, so that one team's loads, maxima and hand-overs run under the other's exponentials
+        // and the products.  A team takes its 128 x 128 scores into registers at once, which frees their place for the next tile's.  What a
+        // tile needs of the one before it is only the running maximum.
+        // (Measured at 4096 rows by 32768 keys: one tile at a time by eight warps 2.25 ms, by sixteen 2.2; two teams with the scores left in
+        // tensor memory, the weights written over them: 1.94, the two teams in step and the products between them.)
+        const uint32_t quarter = warp & 3, half = warp >> 2 & 1, team = warp >> 3, row = quarter * 32 + lane;
         const uint32_t lane_addr = (quarter * 32) << 16;
-        const uint32_t tok = row / G, hq = row % G;
-        uint32_t g = 0, tc = 0;
-        bool ok = true;
-        while (walk.next(it)) {
-            const bool live = tok < it.ntok && row < tpt * G;
-            const int32_t lim = it.lim0 + int32_t(tok);
-            if (ok && !mbar_wait(q_full, tc & 1, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
+        uint32_t g = 0, met = 0, all = 0; // tiles, meetings of the pair, of all warps, so far
+        for (uint32_t ni = 0;; ni++) {
+            PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+            const uint32_t kt0 = items[ni % kPpItems].kt0, kt1 = items[ni % kPpItems].kt1;
+            if (kt0 == kt1) break;
+            const int32_t lim0 = items[ni % kPpItems].lim0;
+            const int32_t lim = lim0 + int32_t(row / a.group);
+            PP_WAIT(q_full, ni & 1, kStatusFullTimeout);
             const float rs = __uint_as_float(uint32_t(row_e[row]) << 23) * a.scale_log2;
             __syncwarp();
             if (lane == 0) mbar_arrive(q_empty); // the factor has been read
-            float m = -INFINITY, l = 0.f;
-            for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
+            float m = -INFINITY, l = 0.f; // the maximum that l goes by
+            for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
+                if ((g & 1) != team) continue;
                 const int32_t key0 = int32_t(kt * kPpKeys + half * 64);
                 const uint32_t ss = g % kPpScaleRing, pb = g % NP;
-                if (ok && !mbar_wait(&sc_full[ss], (g / kPpScaleRing) & 1, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
-                float c[4], lv[4], iv[4];
-                bool bad = false;
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const float4 v = scl[ss * 8 + half * 4 + b];
-                    c[b] = v.x * rs, lv[b] = v.y, iv[b] = v.z;
-                    bad |= v.w != 0.f;
-                }
-                uint32_t badmask = 0;
-                if (bad) {
-#pragma unroll
-                    for (int b = 0; b < 4; b++) badmask |= (scl[ss * 8 + half * 4 + b].w != 0.f ? 1u : 0u) << b;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sc_empty[ss]);
-                if (ok && !mbar_wait(s_full, g & 1, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
+                PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1, kStatusFullTimeout);
+                const float2 *sc = scl + ss * kPpScales + half * 4;
+                PP_WAIT(&s_full[team], g >> 1 & 1, kStatusFullTimeout);
                 tc_fence_after();
-                uint32_t sr[2][32];
-                tmem_ld32(tmem_s + lane_addr + half * 64, sr[0]);
-                tmem_ld32(tmem_s + lane_addr + half * 64 + 32, sr[1]);
+                uint32_t s[2][32];
+                tmem_ld32(tmem_s + lane_addr + half * 64, s[0]);
+                tmem_ld32(tmem_s + lane_addr + half * 64 + 32, s[1]);
                 tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_free); // the scores are in registers
-                float s[64];
-#pragma unroll
-                for (int k = 0; k < 64; k++) s[k] = __uint_as_float(sr[k >> 5][k & 31]);
-                if (key0 + 64 > it.lim0 || badmask) {
-#pragma unroll
-                    for (int k = 0; k < 64; k++)
-                        if (key0 + k >= lim || (badmask >> (k >> 4) & 1)) s[k] = -INFINITY;
+                if (key0 + 64 > lim0) {
+                    mask32(s[0], lim - key0);
+                    mask32(s[1], lim - key0 - 32);
                 }
                 float mx = -INFINITY;
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    float t[4] = {s[b * 16], s[b * 16 + 1], s[b * 16 + 2], s[b * 16 + 3]};
+                    const float f = sc[b].x;
+                    if (f < 0.f) { // a bad block: what its place in shared memory held before
 #pragma unroll
-                    for (int k = 4; k < 16; k++) t[k & 3] = fmaxf(t[k & 3], s[b * 16 + k]);
-                    mx = fmaxf(mx, fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c[b], lv[b]));
+                        for (int k = 0; k < 16; k++) s[b >> 1][(b & 1) * 16 + k] = 0xff800000u;
+                    }
+                    const float *x = reinterpret_cast<const float *>(&s[b >> 1][(b & 1) * 16]);
+                    float t[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
+                    t[0] = max3(t[0], x[6], x[7]), t[1] = max3(t[1], x[8], x[9]), t[0] = max3(t[0], x[10], x[11]), t[1] = max3(t[1], x[12], x[13]);
+                    mx = fmaxf(mx, fmaxf(max3(t[0], x[14], x[15]), t[1]) * (fabsf(f) * rs));
                 }
-                // the two threads of a row agree on one maximum; rounded up it is still one that no score passes
-                __nv_bfloat16 *x = xch + (g & 1) * 256;
-                const __nv_bfloat16 up = __float2bfloat16_ru(mx);
-                x[half * 128 + row] = up;
-                pair_sync(quarter);
-                mx = fmaxf(__bfloat162float(up), __bfloat162float(x[(half ^ 1) * 128 + row]));
-                const bool need = mx > m + kPpRescale;
-                float f = 1.f;
-                if (need) {
-                    f = ex2_approx(m - mx); // 0 for the first
-                    m = mx;
-                    l *= f;
+                // the two threads of a row agree on one maximum (rounded up it is still one that no score passes), and with the other
+                // team's of the tile before
+                __nv_bfloat16 *x = xch + team * 256;
+                x[half * 128 + row] = __float2bfloat16_ru(mx);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pair_met[team * 4 + quarter]);
+                float m_was = -INFINITY;
+                if (kt > kt0) {
+                    PP_WAIT(&m_full[((g - 1) & 1) * 4 + quarter], (g - 1) >> 1 & 1, kStatusMmaTimeout);
+                    m_was = __bfloat162float(mpub[((g - 1) & 1) * 128 + row]);
                 }
-                if (kt > it.kt0 && __any_sync(0xffffffffu, need)) {
-                    // the product of the tile before must have landed in O
-                    const uint32_t gp = g - 1;
-                    if (ok && !mbar_wait(&pv_done[gp % NP], (gp / NP) & 1, abort_flag)) { give_up(kStatusMmaTimeout); ok = false; }
+                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1, kStatusMmaTimeout);
+                const float top = fmaxf(__bfloat162float(x[row]), __bfloat162float(x[128 + row]));
+                const bool need = __any_sync(0xffffffffu, top > m_was + kPpRescale);
+                const float mt = need ? fmaxf(m_was, __bfloat162float(__float2bfloat16_ru(top + kPpSpare))) : m_was;
+                if (half == 0) mpub[(g & 1) * 128 + row] = __float2bfloat16(mt);
+                __syncwarp();
+                if (lane == 0) {
+                    if (half == 0) mbar_arrive(&m_full[(g & 1) * 4 + quarter]);
+                    mbar_arrive(&pair_met[team * 4 + quarter]); // this tile's maxima have been read
+                }
+                if (mt != m) { // (also where the other team has moved it)
+                    l *= ex2_approx(m - mt); // 0 for the first
+                    m = mt;
+                }
+                const float fv = scl[ss * kPpScales + 8].x;
+                if (kt > kt0 && (need || fv != 1.f)) {
+                    // The product of the tile before must have landed in O.  (That of two tiles before first: it shares no barrier with it, and
+                    // once it is done the barrier waited for next is in the phase asked for or the one before.)
+                    if (g >= 2 && NP == 2) PP_WAIT(&pv_done[g & 1], (g - 2) >> 1 & 1, kStatusMmaTimeout);
+                    PP_WAIT(&pv_done[(g - 1) & 1], (g - 1) >> 1 & 1, kStatusMmaTimeout);
                     tc_fence_after();
+                    const float f = (mt != m_was ? ex2_approx(m_was - mt) : 1.f) * fv;
 #pragma unroll 1
-                    for (int k = 0; k < D / 2; k += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(tmem_o + lane_addr + half * (D / 2) + k, o);
+                    for (int k = 0; k < D / 2; k += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(tmem_o + lane_addr + half * (D / 2) + k, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        tmem_st32(tmem_o + lane_addr + half * (D / 2) + k, o);
+                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st16(tmem_o + lane_addr + half * (D / 2) + k, o);
                     }
                     tmem_wait_st();
                 }
-                const float base = kPpShift - (m == -INFINITY ? 0.f : m);
-                uint32_t pw[PARTS][16];
+                const float base = kPpShift + kPpHalf - (m == -INFINITY ? 0.f : m);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const float d = lv[b] + base;
-                    float sum[2] = {0.f, 0.f};
+                for (int h = 0; h < 3; h++) {
+                    // the exponentials of 32 keys, and between them the terms of the 32 before: the two run on different units
+                    uint32_t pw[PARTS][8];
 #pragma unroll
-                    for (int k = 0; k < 16; k += 4) {
-                        float e[4];
+                    for (int q = 0; q < 8; q++) {
+                        if (h < 2) {
+                            float *e = reinterpret_cast<float *>(&s[h][q * 4]);
+                            const float2 f = sc[h * 2 + (q >> 2)];
+                            const float c = fabsf(f.x) * rs, d = f.y + base;
+                            const float2 t0 = fma2(make_float2(e[0], e[1]), make_float2(c, c), make_float2(d, d));
+                            const float2 t1 = fma2(make_float2(e[2], e[3]), make_float2(c, c), make_float2(d, d));
+                            e[0] = ex2_approx(t0.x), e[1] = ex2_approx(t0.y), e[2] = ex2_approx(t1.x), e[3] = ex2_approx(t1.y);
+                        }
+                        if (h > 0) {
+                            const float *e = reinterpret_cast<const float *>(&s[h - 1][q * 4]);
+                            uint32_t w[PARTS];
+                            split_weights<PARTS>(e, w);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) e[j] = ex2_approx(fmaf(s[b * 16 + k + j], c[b], d));
-                        sum[0] += e[0] + e[1], sum[1] += e[2] + e[3];
-                        uint32_t w[PARTS];
-                        split4<PARTS>(e[0], e[1], e[2], e[3], w);
-#pragma unroll
-                        for (int p = 0; p < PARTS; p++) pw[p][b * 4 + k / 4] = w[p];
+                            for (int p = 0; p < PARTS; p++) pw[p][q] = w[p];
+                            sum[q & 1] = add2(sum[q & 1], add2(make_float2(e[0], e[1]), make_float2(e[2], e[3])));
+                            if (q & 2 && q & 1) {
+                                const float2 t = add2(sum[0], sum[1]);
+                                l = fmaf(t.x + t.y, ex2_approx(-sc[(h - 1) * 2 + (q >> 2)].y), l);
+                                sum[0] = sum[1] = make_float2(0.f, 0.f);
+                            }
+                        }
                     }
-                    l = fmaf(sum[0] + sum[1], iv[b], l);
-                }
-                // P buffer: the product of NP tiles ago has read it
-                if (ok && !mbar_wait(&pv_done[pb], ((g / NP) & 1) ^ 1, abort_flag)) { give_up(kStatusMmaTimeout); ok = false; }
-                tc_fence_after();
+                    if (h == 1 && g >= uint32_t(NP)) { // the product of NP tiles ago has read this buffer (pv_done: a barrier for even and one for odd tiles)
+                        PP_WAIT(&pv_done[(g - NP) & 1], (g - NP) >> 1 & 1, kStatusMmaTimeout);
+                        tc_fence_after();
+                    }
+                    if (h > 0) {
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) tmem_st16(tmem_p + lane_addr + pb * L::kPCols + p * 32 + half * 16, pw[p]);
+                        for (int p = 0; p < PARTS; p++) tmem_st8(tmem_p + lane_addr + pb * L::kPCols + p * 32 + half * 16 + (h - 1) * 8, pw[p]);
+                    }
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[pb]);
+                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1, kStatusMmaTimeout); // (long over)
             }
-            // ---- the tile's end: two halves of a row's sum become one, O leaves tensor memory
-            softmax_sync(); // every warp has read its last maxima: the sums take their place
-            lx[half * 128 + row] = l;
-            softmax_sync();
-            l += lx[(half ^ 1) * 128 + row];
-            softmax_sync();
-            if (ok && !mbar_wait(o_final, tc & 1, abort_flag)) { give_up(kStatusMmaTimeout); ok = false; }
+            // ---- the tile's end: the four sums of a row become one, O leaves tensor memory
+#define PP_MEET_ALL()                                      \
+    __syncwarp();                                          \
+    if (lane == 0) mbar_arrive(all_met);                   \
+    PP_WAIT(all_met, all++ & 1, kStatusMmaTimeout)
+            PP_MEET_ALL(); // the last tile's maximum is there; the exchange area is free for the sums
+            const float vref = scl[((g - 1) % kPpScaleRing) * kPpScales + 8].y;
+            {
+                const float mt = __bfloat162float(mpub[((g - 1) & 1) * 128 + row]);
+                if (mt != m) l *= ex2_approx(m - mt);
+                m = mt;
+            }
+            if (half) lx[team * 128 + row] = l;
+            PP_MEET_ALL();
+            if (!half) l += lx[team * 128 + row];
+            PP_MEET_ALL();
+            if (!half) lx[team * 128 + row] = l;
+            PP_MEET_ALL();
+            l = (lx[row] + lx[128 + row]) * 256.f; // (the weights' sums were taken times 2^-8)
+            PP_MEET_ALL();
+            const PpItem &it = items[ni % kPpItems];
+            const uint32_t cq = warp >> 2, tok = row / a.group, hq = row % a.group;
+            const bool live = tok < it.ntok && row < tpt * a.group;
+            const uint32_t parts = it.parts;
+            const size_t orow = live ? size_t(it.row0 + tok) * a.heads + it.head * a.group + hq : 0;
+            const uint32_t c0 = it.c0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
+            PP_WAIT(o_final, ni & 1, kStatusMmaTimeout);
             tc_fence_after();
-            const bool whole = it.kt0 == 0 && it.kt1 == it.tiles;
-            const size_t orow = live ? size_t(it.q.row0 + it.tok0 + tok) * a.heads + it.head * G + hq : 0;
             auto finish = [&](int d, float4 v, float inv) { // dims d .. d + 3 of this thread's row
                 v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
                 if (a.q_and_gate) {
@@ -477,83 +687,96 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 paged_store4(a, orow * D + d, v.x, v.y, v.z, v.w);
             };
             auto inverse = [](float sum) { return sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); }; // no key: 0; NaN stays
-            float *part = a.parts + (size_t(blockIdx.x) * 2 + (it.kt0 == 0 ? 1 : 0)) * a.part_floats;
-            const float inv = inverse(l);
+            float *part = a.parts + (size_t(blockIdx.x) * 2 + (kt0 == 0 ? 1 : 0)) * a.part_floats;
+            const float inv = inverse(l) * vref;
 #pragma unroll 1
-            for (int k = 0; k < D / 2; k += 32) {
-                uint32_t o[32];
-                tmem_ld32(tmem_o + lane_addr + half * (D / 2) + k, o);
+            for (int k = 0; k < D / 4; k += 16) {
+                uint32_t o[16];
+                tmem_ld16(tmem_o + lane_addr + cq * (D / 4) + k, o);
                 tmem_wait_ld();
-                if (k + 32 >= D / 2) {
+                if (k + 16 >= D / 4) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(o_empty);
                 }
                 if (live) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
+                    for (int j = 0; j < 16; j += 4) {
                         const float4 v = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
-                        const int d = half * (D / 2) + k + j;
-                        if (whole) finish(d, v, inv);
+                        const int d = cq * (D / 4) + k + j;
+                        if (parts == 1) finish(d, v, inv);
                         else *reinterpret_cast<float4 *>(part + size_t(row) * D + d) = v;
                     }
                 }
             }
-            if (!whole) {
-                if (half == 0) *reinterpret_cast<float2 *>(part + kPpRows * D + row * 2) = make_float2(m, l);
+            if (parts > 1) {
+                if (cq == 0) *reinterpret_cast<float2 *>(part + kPpRows * D + row * 2) = make_float2(m, l);
+                if (warp == 0 && lane == 0) part[kPpRows * (D + 2)] = vref;
                 // the last CTA of the item to arrive joins the parts, in the order of the CTAs
-                const uint32_t c0 = paged_cta_of(sh, it.first), c1 = paged_cta_of(sh, it.first + it.tiles - 1), parts = c1 - c0 + 1;
-                uint32_t *counter = a.words + kPagedCounters + c0;
                 __threadfence();
-                softmax_sync();
-                if (threadIdx.x == 0) {
+                PP_MEET_ALL();
+                if (warp == 0 && lane == 0) {
+                    uint32_t *counter = a.words + kPagedCounters + c0;
                     const uint32_t n = atomicAdd(counter, 1);
                     if (n + 1 == parts) *counter = 0;
                     *arrived = n + 1;
                 }
-                softmax_sync();
-                if (*arrived == parts) {
+                PP_MEET_ALL();
+                const bool last = *arrived == parts;
+                PP_MEET_ALL(); // `arrived` has been read
+                if (last && live) {
                     __threadfence();
-                    if (live) {
-                        auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
-                        float top = -INFINITY, sum = 0.f;
-                        for (uint32_t p = 0; p < parts; p++) top = fmaxf(top, __ldcg(part_of(p) + kPpRows * D + row * 2));
-                        const float mu = top == -INFINITY ? 0.f : top;
-                        for (uint32_t p = 0; p < parts; p++) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(p) + kPpRows * D + row * 2));
-                            sum += ml.y * ex2_approx(ml.x - mu);
-                        }
-                        const float is = inverse(sum);
+                    auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
+                    float top = -INFINITY, sum = 0.f;
+                    #pragma unroll 1
+                    for (uint32_t p = 0; p < parts; p++) top = fmaxf(top, __ldcg(part_of(p) + kPpRows * D + row * 2));
+                    const float mu = top == -INFINITY ? 0.f : top;
+                    float vtop = 0.f;
 #pragma unroll 1
-                        for (int k = 0; k < D / 2; k += 16) {
-                            const int d = half * (D / 2) + k;
-                            float4 v[4];
+                    for (uint32_t p = 0; p < parts; p++) vtop = fmaxf(vtop, __ldcg(part_of(p) + kPpRows * (D + 2)));
+#pragma unroll 1
+                    for (uint32_t p = 0; p < parts; p++) {
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(p) + kPpRows * D + row * 2));
+                        sum += ml.y * ex2_approx(ml.x - mu);
+                    }
+                    const float is = inverse(sum) * vtop;
+#pragma unroll 1
+                    for (int k = 0; k < D / 4; k += 16) {
+                        const int d = cq * (D / 4) + k;
+                        float4 v[4];
 #pragma unroll
-                            for (int j = 0; j < 4; j++) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            for (uint32_t p = 0; p < parts; p++) {
-                                const float *pp = part_of(p);
-                                const float wt = ex2_approx(__ldcg(pp + kPpRows * D + row * 2) - mu);
+                        for (int j = 0; j < 4; j++) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                        for (uint32_t p = 0; p < parts; p++) {
+                            const float *pp = part_of(p);
+                            const float wt = ex2_approx(__ldcg(pp + kPpRows * D + row * 2) - mu) * (__ldcg(pp + kPpRows * (D + 2)) / vtop);
 #pragma unroll
-                                for (int j = 0; j < 4; j++) {
-                                    const float4 u = __ldcg(reinterpret_cast<const float4 *>(pp + size_t(row) * D + d + 4 * j));
-                                    v[j].x = fmaf(u.x, wt, v[j].x), v[j].y = fmaf(u.y, wt, v[j].y), v[j].z = fmaf(u.z, wt, v[j].z), v[j].w = fmaf(u.w, wt, v[j].w);
-                                }
+                            for (int j = 0; j < 4; j++) {
+                                const float4 u = __ldcg(reinterpret_cast<const float4 *>(pp + size_t(row) * D + d + 4 * j));
+                                v[j].x = fmaf(u.x, wt, v[j].x), v[j].y = fmaf(u.y, wt, v[j].y), v[j].z = fmaf(u.z, wt, v[j].z), v[j].w = fmaf(u.w, wt, v[j].w);
                             }
-#pragma unroll
-                            for (int j = 0; j < 4; j++) finish(d + 4 * j, v[j], is);
                         }
+#pragma unroll
+                        for (int j = 0; j < 4; j++) finish(d + 4 * j, v[j], is);
                     }
                 }
-                softmax_sync(); // `arrived` has been read
             }
-            tc++;
         }
     }
-
+done:
+    if (warp == 20) { // what was issued lands before the shared memory goes (it has, unless a wait gave up)
+        for (uint32_t k = copied_k > NK ? copied_k - NK : 0; k < copied_k; k++) mbar_wait(&k_full[k % NK], (k / NK) & 1, never_set, 200000u);
+        for (uint32_t k = copied_v > NV ? copied_v - NV : 0; k < copied_v; k++) mbar_wait(&v_full[k % NV], (k / NV) & 1, never_set, 200000u);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 13) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    __syncwarp();
+    if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+#undef PP_WAIT_FOR
+#undef PP_WAIT_AHEAD
+#undef PP_WAIT
+#undef PP_MEET_ALL
 }
 
 template <int D, int PARTS>

@@ -8,9 +8,11 @@
 
 namespace saetta {
 
+// (Called, not copied into every caller, as is what divides 64-bit numbers below: the kernels' code has to stay well below the 128 KB
+// that an SM keeps of it; past that every instruction is fetched from far away.)
 // sum over i < n of floor((a i + b) / m): counts lattice points under the line, exchanging slope and modulus as Euclid's
 // algorithm does.
-__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+static __device__ __noinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
     uint64_t sum = 0;
     while (true) {
         if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
@@ -47,7 +49,7 @@ struct PagedTiles {
     }
     // at least one tile, so that rows that see no key are written too
     __device__ __forceinline__ uint32_t count(const PagedSeq &q, uint32_t r) const { return max(1u, (keys(q, r) + T - 1) / T); }
-    __device__ __forceinline__ uint64_t before(const PagedSeq &q, uint32_t r) const { // of row tiles 0 .. r - 1
+    __device__ __noinline__ uint64_t before(const PagedSeq &q, uint32_t r) const { // of row tiles 0 .. r - 1
         if (!r) return 0;
         if (q.kv < q.n) return uint64_t(r) * count(q, 0);
         const uint32_t full = r == row_tiles(q) ? r - 1 : r;
@@ -65,7 +67,7 @@ struct PagedItem {
     uint32_t tok0, ntok;        // tokens of the row tile, in the sequence
     int32_t lim0;               // keys the tile's first token sees (<= 0: none)
     uint32_t tiles, kt0, kt1;   // key tiles of the item, and this CTA's [kt0, kt1)
-    uint64_t first;             // flat index of the item's tile 0
+    uint32_t at;                // tile kt0's place in the CTA's share
 };
 
 struct PagedShare {
@@ -80,35 +82,34 @@ template <int T>
 struct PagedWalk {
     const PagedArgs &a;
     PagedTiles<T> tiles;
-    uint64_t x, x1;
-    uint32_t seq, head, rtile, rtiles;
+    uint32_t at, end; // places in the share
+    uint32_t seq, head, rtile, rtiles, kt0;
     PagedSeq q;
-    uint32_t kt0;
 
     __device__ __forceinline__ PagedWalk(const PagedArgs &args, const PagedShare &s, uint32_t tpt) : a(args), tiles{tpt} {
-        x = s.x0, x1 = s.x1, seq = s.seq, head = s.head, rtile = s.rtile, kt0 = 0, rtiles = 0;
-        if (x < x1) {
+        at = 0, end = uint32_t(s.x1 - s.x0), seq = s.seq, head = s.head, rtile = s.rtile, kt0 = 0, rtiles = 0;
+        if (end) {
             q = paged_seq(a, seq);
             rtiles = tiles.row_tiles(q);
-            kt0 = uint32_t(x - (s.head_base + uint64_t(head) * tiles.per_head(q) + tiles.before(q, rtile)));
+            kt0 = uint32_t(s.x0 - (s.head_base + uint64_t(head) * tiles.per_head(q) + tiles.before(q, rtile)));
         }
     }
     __device__ __forceinline__ bool next(PagedItem &it) {
-        if (x >= x1) return false;
+        if (at >= end) return false;
         it.seq = seq, it.head = head, it.rtile = rtile, it.q = q;
         it.tok0 = rtile * tiles.tpt, it.ntok = min(tiles.tpt, q.n - it.tok0);
         it.lim0 = int32_t(q.kv) - int32_t(q.n) + int32_t(it.tok0) + 1;
         it.tiles = tiles.count(q, rtile);
         it.kt0 = kt0;
-        it.kt1 = uint32_t(min(uint64_t(it.tiles), kt0 + (x1 - x)));
-        it.first = x - kt0;
-        x += it.kt1 - it.kt0;
+        it.kt1 = kt0 + min(it.tiles - kt0, end - at);
+        it.at = at;
+        at += it.kt1 - it.kt0;
         kt0 = 0;
         if (++rtile == rtiles) {
             rtile = 0;
             if (++head == a.kv_heads) {
                 head = 0;
-                if (x < x1)
+                if (at < end)
                     do q = paged_seq(a, ++seq);
                     while (!q.n);
                 rtiles = tiles.row_tiles(q);
@@ -118,12 +119,21 @@ struct PagedWalk {
     }
 };
 
+// Keys that an item's last token sees.
+__device__ __forceinline__ int32_t paged_visible(const PagedItem &it) { return min(int32_t(it.q.kv), it.lim0 + int32_t(it.ntok) - 1); }
+
 // The CTA whose share holds tile x.
-__device__ __forceinline__ uint32_t paged_cta_of(const PagedShare &s, uint64_t x) {
-    uint64_t c = x * s.ctas / s.total;
-    while (s.total * (c + 1) / s.ctas <= x) c++;
-    while (s.total * c / s.ctas > x) c--;
+static __device__ __noinline__ uint32_t paged_cta_of(uint64_t total, uint32_t ctas, uint64_t x) {
+    uint64_t c = x * ctas / total;
+    while (total * (c + 1) / ctas <= x) c++;
+    while (total * c / ctas > x) c--;
     return uint32_t(c);
+}
+// The CTAs that an item's tiles lie in: the first, and how many.
+__device__ __forceinline__ uint2 paged_ctas_of(const PagedShare &s, const PagedItem &it) {
+    const uint64_t first = s.x0 + it.at - it.kt0;
+    const uint32_t c0 = paged_cta_of(s.total, s.ctas, first);
+    return make_uint2(c0, paged_cta_of(s.total, s.ctas, first + it.tiles - 1) - c0 + 1);
 }
 
 // Finds this CTA's share.  All `threads` threads of the block call it; `scratch` (40 words of 8 bytes) and `share` are shared memory.
@@ -132,6 +142,7 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
     const PagedTiles<T> tiles{tpt};
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
     uint64_t total = 0, x0 = 0;
+#pragma unroll 1
     for (int pass = 0; pass < 2; pass++) { // the sum first, then who holds x0
         uint64_t carry = 0;
         for (uint32_t base = 0; base < a.seqs; base += threads) {
@@ -150,6 +161,7 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
             if (lane == 31) scratch[warp] = v;
             __syncthreads();
             uint64_t before = carry, all = 0;
+#pragma unroll 1
             for (uint32_t w = 0; w < warps; w++) {
                 if (w < warp) before += scratch[w];
                 all += scratch[w];

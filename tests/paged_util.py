@@ -88,7 +88,8 @@ def ref_assign(lens, new, finished, free, count, tables, block, rows_cap):
 def ref_attend(q, keys, values, scales, tables, starts, kv_lens, block, scale, gate=None):
     """q f64 [rows][heads][dim]; codes, scales as in ref_store.  Returns (out, bounds): `bounds` holds, per
     (row, head), what the error bounds of the kernels go by: absv (the average of |v| under the weights), mag (the largest scale * sum of
-    |q k|), top (the largest |s|), wide (largest weight times value scale, times the sum of |code|), qwide (largest |q| times the largest
+    |q k|), top (the largest |s|), wide (largest weight, times the
+    sequence's largest value scale, times the sum of |code|), qwide (largest |q| times the largest
     scale * sum of |k|)."""
     rows, heads, dim = q.shape
     kv_heads = keys.shape[1]
@@ -120,7 +121,7 @@ def ref_attend(q, keys, values, scales, tables, starts, kv_lens, block, scale, g
             mag[at], top[at] = a.max(-1), aw.max(-1)
             qwide[at] = np.abs(qs).max(-1) * scale * np.abs(k).sum(-1).max()
             vs = np.repeat(scales[pages, h, 1], block)[:kv]
-            wide[at] = (p * vs).max(-1)[..., None] * np.einsum("ngk,kd->ngd", ~hidden[:, None] & np.ones((1, G, 1), bool), np.abs(v / vs[:, None]))
+            wide[at] = p.max(-1)[..., None] * vs.max() * np.einsum("ngk,kd->ngd", ~hidden[:, None] & np.ones((1, G, 1), bool), np.abs(v / vs[:, None]))
     if gate is not None:
         g = 1.0 / (1.0 + np.exp(-gate))
         out, absv, wide = out * g, absv * g, wide * g

@@ -222,13 +222,14 @@ def bound(out_dt, q_dt, out, b, kv_max, dim, many):
     be off by one part in 2^23 of the sum of |q k|; scale factors and the exponential, a few parts in 2^23 of |s|.  Few rows: a
     probability is a binary16 (2^-11).  Many rows: q and the probabilities are sums of e4m3 values, two (2^-8 of the value) for bfloat16 q,
     three (2^-12) else; below e4m3's normal range a term is off by up to 2^-10 of its unit, where a row's largest q is 2^7 units at least and
-    the largest weight 2^5.5 (it is kept times 2^6, under a maximum that is rounded up to bfloat16: |t| < 64 here)."""
+    the largest weight 2^4.75 of the largest value scale's (it is kept times 2^5.5, under a maximum with half a doubling to spare that is
+    rounded up to bfloat16: |s| < 64 here)."""
     ds = (dim * 2.0 ** -23 + (2.0 ** -11 if q_dt == sa.F32 else 0.0)) * b["mag"] + 8 * 2.0 ** -23 * (b["top"] + 1)
     p_step, floor = 2.0 ** -11, 0.0
     if many:
         ds = ds + 2.0 ** -17 * b["qwide"]
         p_step = 2.0 ** -8 if q_dt == sa.BF16 else 2.0 ** -12 + 2.0 ** -24
-        floor = 2.0 ** -15.5 * b["wide"]
+        floor = 2.0 ** -14.75 * b["wide"]
     rel = p_step + 2 * ds + kv_max * 2.0 ** -23 + 2.0 ** -18
     return (U[out_dt] * np.abs(out) + (rel[..., None] * b["absv"] + floor) * (1 + U[out_dt]) + 2.0 ** -24 * (out_dt == sa.F16) + 1e-30)
 
