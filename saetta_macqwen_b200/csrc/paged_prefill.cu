@@ -48,31 +48,31 @@ struct PpLayout {
     static_assert(kSmem <= 227 * 1024, "fits a CTA's shared memory");
 };
 
-// The products are issued by whole warps in step, one lane's predicate inside the instruction, from operands that are the same in every
-// lane as far as the compiler can tell (uniform()): under a branch of one lane it takes 120 clocks to bring the operands of each product to
-// the registers that the instruction reads, and the pipe needs 64 for the product.
+// The products are issued under elect.sync's predicate, which the compiler knows to be one lane of a warp in step: five instructions each,
+// from uniform registers.  (Under `lane == 0`, or with the predicate inside the instruction, 15 to 27, and 120 clocks for each product, of which the
+// pipe needs 64.)
 // Descriptors come as their low words; the high word, the same for all (stride 1024 bytes, 128-byte swizzle), is an immediate.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ void tc_mma8(uint32_t leader, uint32_t d_tmem, uint32_t adesc, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(yes));
+    return yes;
+}
+__device__ __forceinline__ void tc_mma8(uint32_t d_tmem, uint32_t adesc, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(adesc), "r"(bdesc), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(adesc), "r"(bdesc), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
         : "memory");
 }
 // A from tensor memory: row m in lane m, four e4m3 values in a column.
-__device__ __forceinline__ void tc_mma8_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma8_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 b, {%2, %5};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], b, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "r"(bdesc), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], b, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(bdesc), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
         : "memory");
-}
-__device__ __forceinline__ void tc_commit_if(uint32_t leader, uint64_t *bar) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-                 ::"r"(smem_u32(bar)), "r"(leader)
-                 : "memory");
 }
 __device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3ffffu) >> 4) | (lbo_bytes >> 4) << 16; }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -175,17 +175,18 @@ __device__ __forceinline__ void split_weights(const float *x, uint32_t (&w)[PART
         if (p + 1 < PARTS) h0 = hsub2_u32(h0, h0 & 0xff80ff80u), h1 = hsub2_u32(h1, h1 & 0xff80ff80u);
     }
 }
-// A bounded wait of a whole warp, in few instructions (there are forty of them): by polls, each of which the hardware holds for a while, up to
-// about a microsecond.  SLEEP: nanoseconds between polls, for roles that run ahead of the others.
-template <int SLEEP>
-__device__ __forceinline__ bool short_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
-    bool ok = true;
-#pragma unroll 1
-    for (uint32_t n = 0; ok && !mbar_test(bar, parity); n++) {
-        if (SLEEP) __nanosleep(SLEEP);
-        if ((n & 63) == 63) ok = n <= 4000000u && !*abort_flag;
-    }
-    return __all_sync(0xffffffffu, ok);
+// A bounded wait of a whole warp, in as few instructions as it takes (there are forty of them): polls that the hardware holds for up to a
+// millisecond each, 2000 at most.
+__device__ __forceinline__ bool short_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 n;\n\tmov.u32 n, 2000;\n"
+        "poll:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000000;\n\t@p bra over;\n\tsub.u32 n, n, 1;\n\t"
+        "setp.ne.u32 p, n, 0;\n\t@p bra poll;\nover:\n\tmov.u32 %0, n;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
 }
 __device__ __forceinline__ float lg2_approx(float x) {
     float y;
@@ -231,7 +232,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
              *p_full = bars + 34, *pv_done = bars + 36, *q_full = bars + 38, *q_empty = bars + 39, *s_free = bars + 40, *o_final = bars + 41,
              *o_empty = bars + 42, *all_met = bars + 43, *pair_met = bars + 44 /* [team][row quarter] */, *m_full = bars + 52 /* [2][4 row quarters] */;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 60);
-    volatile uint32_t *abort_flag = tmem_slot + 1, *never_set = tmem_slot + 2, *arrived = tmem_slot + 3;
+    volatile uint32_t *never_set = tmem_slot + 1, *arrived = tmem_slot + 2;
     uint8_t *row_e = reinterpret_cast<uint8_t *>(bars + 62); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
 
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -248,7 +249,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int s = 0; s < 8; s++) mbar_init(&pair_met[s], 2), mbar_init(&m_full[s], 1);
         mbar_init(q_full, 4), mbar_init(q_empty, 1 + kPpWarps), mbar_init(s_free, kPpWarps / 2), mbar_init(o_final, 1), mbar_init(o_empty, kPpWarps);
         mbar_init(all_met, kPpWarps);
-        *abort_flag = 0, *never_set = 0;
+        *never_set = 0;
         mbar_fence_init();
     }
     pdl_wait();
@@ -263,16 +264,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + L::kTmemO, tmem_s = tmem + L::kTmemS, tmem_p = tmem + L::kTmemP;
-    // Waits are bounded: one that gives up leaves its role, sets the status and the flag that ends the others' waits.  (No role waits at a
-    // named barrier, which would have no bound.)
-#define PP_WAIT_FOR(sleep, bar, parity, bit)            \
-    if (!short_wait<sleep>(bar, parity, abort_flag)) {  \
-        atomicOr(a.words, bit);                         \
-        *abort_flag = 1;                                \
-        goto done;                                      \
-    }
-#define PP_WAIT(bar, parity, bit) PP_WAIT_FOR(0, bar, parity, bit)
-#define PP_WAIT_AHEAD(bar, parity, bit) PP_WAIT_FOR(64, bar, parity, bit)
+    // Waits are bounded: one that gives up ends its role, which ends the others' waits the same way.  (No role waits at a named barrier, which
+    // would have no bound.)
+#define PP_WAIT(bar, parity) \
+    if (!short_wait(bar, parity)) goto failed
 
     uint32_t copied_k = 0, copied_v = 0; // of the copying warp
 
@@ -298,7 +293,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     if (kk == kk1) {
                         PagedItem it;
                         walk.next(it);
-                        PP_WAIT_AHEAD(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1, kStatusEmptyTimeout);
+                        PP_WAIT(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1);
                         const uint2 span = paged_ctas_of(*share, it);
                         kk = it.kt0, kk1 = it.kt1, keys = walk.tiles.keys(it.q, it.rtile), head = it.head;
                         table = a.tables + size_t(it.seq) * a.table_stride;
@@ -320,7 +315,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 const uint32_t dst = slab * (kPpKeys * 128) + page * bt * 128;
                 if (i >= 1 && i <= tiles) {
                     const uint32_t g = i - 1, st = g % NK, n = __popc(__ballot_sync(0xffffffffu, row[1] >= 0));
-                    PP_WAIT(&k_empty[st], (g / NK & 1) ^ 1, kStatusEmptyTimeout);
+                    PP_WAIT(&k_empty[st], (g / NK & 1) ^ 1);
                     if (lane == 0) mbar_expect_tx(&k_full[st], n * bt * 128);
                     copied_k = g + 1;
                     __syncwarp();
@@ -328,14 +323,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
                 if (i >= kPpAhead + 1) {
                     const uint32_t g = i - kPpAhead - 1, st = g % NV, n = __popc(__ballot_sync(0xffffffffu, row[kPpAhead + 1] >= 0));
-                    PP_WAIT(&v_empty[st], (g / NV & 1) ^ 1, kStatusEmptyTimeout);
+                    PP_WAIT(&v_empty[st], (g / NV & 1) ^ 1);
                     if (lane == 0) mbar_expect_tx(&v_full[st], n * bt * 128);
                     copied_v = g + 1;
                     __syncwarp();
                     if (row[kPpAhead + 1] >= 0) tma_load_3d(ring_v + st * L::kStage + dst, &map_v, &v_full[st], 0, row[kPpAhead + 1], int(slab));
                 }
             }
-            PP_WAIT_AHEAD(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1, kStatusEmptyTimeout);
+            PP_WAIT(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1);
             if (lane == 0) {
                 items[ni % kPpItems].kt0 = items[ni % kPpItems].kt1 = 0;
                 mbar_arrive(&item_full[ni % kPpItems]);
@@ -344,35 +339,36 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             // ------------------------------------------------------------ score products
             constexpr uint32_t idesc = (1u << 4) | (uint32_t(kPpKeys >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
             const uint32_t ad = uniform(desc_low(smem_u32(sQ), 16)), bd0 = uniform(desc_low(smem_u32(ring), 16)), ts = uniform(tmem_s);
-            const uint32_t leader = lane == 0;
             uint32_t g = 0;
             for (uint32_t ni = 0;; ni++) {
-                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
                 const uint32_t end = g + uniform(items[ni % kPpItems].kt1 - items[ni % kPpItems].kt0);
                 if (g == end) break;
                 __syncwarp();
-                if (leader) mbar_arrive(&item_empty[ni % kPpItems]);
-                PP_WAIT(q_full, ni & 1, kStatusFullTimeout);
+                if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
+                PP_WAIT(q_full, ni & 1);
                 for (; g < end; g++) {
                     const uint32_t st = g % NK;
-                    PP_WAIT(&k_full[st], g / NK & 1, kStatusFullTimeout);
-                    PP_WAIT(s_free, (g & 1) ^ 1, kStatusMmaTimeout);
+                    PP_WAIT(&k_full[st], g / NK & 1);
+                    PP_WAIT(s_free, (g & 1) ^ 1);
                     tc_fence_after();
                     __syncwarp();
                     const uint32_t bd = bd0 + st * (L::kStage >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (uint32_t k = 0; k < PARTS * D / 32; k++) // 32 dims of one term; slabs of 128 dims lie 16 KB apart, the terms of Q behind one another
-                        tc_mma8(leader, ts, ad + (k >> 2) * 1024 + (k & 3) * 2, bd + (k >> 2) % kSlabs * 1024 + (k & 3) * 2, idesc, k);
-                    tc_commit_if(leader, &s_full[g & 1]);
-                    tc_commit_if(leader, &k_empty[st]);
-                    if (g + 1 == end) tc_commit_if(leader, q_empty);
+                        for (uint32_t k = 0; k < PARTS * D / 32; k++) // 32 dims of one term; slabs of 128 dims lie 16 KB apart, the terms of Q behind one another
+                            tc_mma8(ts, ad + (k >> 2) * 1024 + (k & 3) * 2, bd + (k >> 2) % kSlabs * 1024 + (k & 3) * 2, idesc, k > 0);
+                        tc_commit(&s_full[g & 1]);
+                        tc_commit(&k_empty[st]);
+                        if (g + 1 == end) tc_commit(q_empty);
+                    }
                 }
             }
         } else if (warp == 22) {
             // ------------------------------------------------------------ scales of each 16 keys
             uint32_t g = 0;
             for (uint32_t ni = 0;; ni++) {
-                PP_WAIT_AHEAD(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
                 const PpItem &it = items[ni % kPpItems];
                 const uint32_t keys = it.keys, head = it.head, kt1 = it.kt1;
                 uint32_t kt = it.kt0;
@@ -403,7 +399,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     v.y = good ? fmaxf(lg2_approx(v.y / top), -40.f) : 0.f;
                     if (lane == 8) v = make_float2(vref > 0.f ? vref / top : 1.f, top);
                     vref = top;
-                    PP_WAIT_AHEAD(&sc_empty[ss], (g / kPpScaleRing & 1) ^ 1, kStatusEmptyTimeout);
+                    PP_WAIT(&sc_empty[ss], (g / kPpScaleRing & 1) ^ 1);
                     if (lane < kPpScales) scl[ss * kPpScales + lane] = v;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[ss]);
@@ -413,19 +409,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             // ------------------------------------------------------------ value products
             constexpr uint32_t idesc = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
             const uint32_t bd0 = uniform(desc_low(smem_u32(ring_v), kPpKeys * 128)), to = uniform(tmem_o), tp = uniform(tmem_p);
-            const uint32_t leader = lane == 0;
             uint32_t g = 0;
             for (uint32_t ni = 0;; ni++) {
-                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+                PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
                 const int32_t vis = items[ni % kPpItems].vis;
                 const uint32_t kt0 = uniform(items[ni % kPpItems].kt0), kt1 = uniform(items[ni % kPpItems].kt1);
                 if (kt0 == kt1) break;
                 __syncwarp();
-                if (leader) mbar_arrive(&item_empty[ni % kPpItems]);
+                if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
                 for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
                     const uint32_t st = g % NV, pb = g % NP, ss = g % kPpScaleRing;
-                    PP_WAIT(&v_full[st], g / NV & 1, kStatusFullTimeout);
-                    PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1, kStatusFullTimeout);
+                    PP_WAIT(&v_full[st], g / NV & 1);
+                    PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1);
                     // rows behind the last key, and of bad blocks, may hold NaN, which a weight of 0 does not silence
                     const int32_t key0 = int32_t(kt * kPpKeys);
                     const uint32_t bad = __ballot_sync(0xffffffffu, lane < 8 && scl[ss * kPpScales + (lane & 7)].x < 0.f);
@@ -438,18 +433,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         fence_async_smem();
                         __syncwarp();
                     }
-                    if (kt == kt0) PP_WAIT(o_empty, (ni & 1) ^ 1, kStatusMmaTimeout);
-                    PP_WAIT(&p_full[pb], g / NP & 1, kStatusMmaTimeout);
+                    if (kt == kt0) PP_WAIT(o_empty, (ni & 1) ^ 1);
+                    PP_WAIT(&p_full[pb], g / NP & 1);
                     tc_fence_after();
                     __syncwarp();
                     const uint32_t bd = bd0 + st * (L::kStage >> 4), ap = tp + pb * L::kPCols;
+                    if (elect_one()) {
 #pragma unroll
-                    for (uint32_t k = 0; k < PARTS * kPpKeys / 32; k++) // 32 keys of one term
-                        tc_mma8_ts(leader, to, ap + k * 8, bd + (k & 3) * 256, idesc, (kt - kt0) | k);
-                    tc_commit_if(leader, &pv_done[g & 1]);
-                    tc_commit_if(leader, &v_empty[st]);
-                    tc_commit_if(leader, &sc_empty[ss]); // (its softmax is over too)
-                    if (kt + 1 == kt1) tc_commit_if(leader, o_final);
+                        for (uint32_t k = 0; k < PARTS * kPpKeys / 32; k++) // 32 keys of one term
+                            tc_mma8_ts(to, ap + k * 8, bd + (k & 3) * 256, idesc, k ? 1u : kt - kt0);
+                        tc_commit(&pv_done[g & 1]);
+                        tc_commit(&v_empty[st]);
+                        tc_commit(&sc_empty[ss]); // (its softmax is over too)
+                        if (kt + 1 == kt1) tc_commit(o_final);
+                    }
                 }
             }
         }
@@ -458,7 +455,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         // ------------------------------------------------------------ a tile's Q rows, a thread for each
         const uint32_t row = threadIdx.x - 512, tok = row / a.group, hq = row % a.group;
         for (uint32_t ni = 0;; ni++) {
-            PP_WAIT_AHEAD(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+            PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
             const PpItem &it = items[ni % kPpItems];
             if (it.kt0 == it.kt1) break;
             const bool live = tok < it.ntok && row < tpt * a.group;
@@ -479,7 +476,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const int e = min(max(int(__float_as_uint(top) >> 23), 8), 247) - 134;
             const float up = __uint_as_float(uint32_t(127 - e) << 23);
             // the products of the tile before have read the old Q, and its softmax the old factors
-            PP_WAIT_AHEAD(q_empty, (ni & 1) ^ 1, kStatusMmaTimeout);
+            PP_WAIT(q_empty, (ni & 1) ^ 1);
             row_e[row] = uint8_t(127 + e);
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -517,12 +514,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const uint32_t lane_addr = (quarter * 32) << 16;
         uint32_t g = 0, met = 0, all = 0; // tiles, meetings of the pair, of all warps, so far
         for (uint32_t ni = 0;; ni++) {
-            PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1, kStatusFullTimeout);
+            PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
             const uint32_t kt0 = items[ni % kPpItems].kt0, kt1 = items[ni % kPpItems].kt1;
             if (kt0 == kt1) break;
             const int32_t lim0 = items[ni % kPpItems].lim0;
             const int32_t lim = lim0 + int32_t(row / a.group);
-            PP_WAIT(q_full, ni & 1, kStatusFullTimeout);
+            PP_WAIT(q_full, ni & 1);
             const float rs = __uint_as_float(uint32_t(row_e[row]) << 23) * a.scale_log2;
             __syncwarp();
             if (lane == 0) mbar_arrive(q_empty); // the factor has been read
@@ -531,9 +528,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 if ((g & 1) != team) continue;
                 const int32_t key0 = int32_t(kt * kPpKeys + half * 64);
                 const uint32_t ss = g % kPpScaleRing, pb = g % NP;
-                PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1, kStatusFullTimeout);
+                PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1);
                 const float2 *sc = scl + ss * kPpScales + half * 4;
-                PP_WAIT(&s_full[team], g >> 1 & 1, kStatusFullTimeout);
+                PP_WAIT(&s_full[team], g >> 1 & 1);
                 tc_fence_after();
                 uint32_t s[2][32];
                 tmem_ld32(tmem_s + lane_addr + half * 64, s[0]);
@@ -567,10 +564,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 if (lane == 0) mbar_arrive(&pair_met[team * 4 + quarter]);
                 float m_was = -INFINITY;
                 if (kt > kt0) {
-                    PP_WAIT(&m_full[((g - 1) & 1) * 4 + quarter], (g - 1) >> 1 & 1, kStatusMmaTimeout);
+                    PP_WAIT(&m_full[((g - 1) & 1) * 4 + quarter], (g - 1) >> 1 & 1);
                     m_was = __bfloat162float(mpub[((g - 1) & 1) * 128 + row]);
                 }
-                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1, kStatusMmaTimeout);
+                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1);
                 const float top = fmaxf(__bfloat162float(x[row]), __bfloat162float(x[128 + row]));
                 const bool need = __any_sync(0xffffffffu, top > m_was + kPpRescale);
                 const float mt = need ? fmaxf(m_was, __bfloat162float(__float2bfloat16_ru(top + kPpSpare))) : m_was;
@@ -588,8 +585,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 if (kt > kt0 && (need || fv != 1.f)) {
                     // The product of the tile before must have landed in O.  (That of two tiles before first: it shares no barrier with it, and
                     // once it is done the barrier waited for next is in the phase asked for or the one before.)
-                    if (g >= 2 && NP == 2) PP_WAIT(&pv_done[g & 1], (g - 2) >> 1 & 1, kStatusMmaTimeout);
-                    PP_WAIT(&pv_done[(g - 1) & 1], (g - 1) >> 1 & 1, kStatusMmaTimeout);
+                    if (g >= 2 && NP == 2) PP_WAIT(&pv_done[g & 1], (g - 2) >> 1 & 1);
+                    PP_WAIT(&pv_done[(g - 1) & 1], (g - 1) >> 1 & 1);
                     tc_fence_after();
                     const float f = (mt != m_was ? ex2_approx(m_was - mt) : 1.f) * fv;
 #pragma unroll 1
@@ -634,7 +631,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         }
                     }
                     if (h == 1 && g >= uint32_t(NP)) { // the product of NP tiles ago has read this buffer (pv_done: a barrier for even and one for odd tiles)
-                        PP_WAIT(&pv_done[(g - NP) & 1], (g - NP) >> 1 & 1, kStatusMmaTimeout);
+                        PP_WAIT(&pv_done[(g - NP) & 1], (g - NP) >> 1 & 1);
                         tc_fence_after();
                     }
                     if (h > 0) {
@@ -646,13 +643,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[pb]);
-                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1, kStatusMmaTimeout); // (long over)
+                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1); // (long over)
             }
             // ---- the tile's end: the four sums of a row become one, O leaves tensor memory
 #define PP_MEET_ALL()                                      \
     __syncwarp();                                          \
     if (lane == 0) mbar_arrive(all_met);                   \
-    PP_WAIT(all_met, all++ & 1, kStatusMmaTimeout)
+    PP_WAIT(all_met, all++ & 1)
             PP_MEET_ALL(); // the last tile's maximum is there; the exchange area is free for the sums
             const float vref = scl[((g - 1) % kPpScaleRing) * kPpScales + 8].y;
             {
@@ -676,7 +673,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const uint32_t c0 = it.c0;
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
-            PP_WAIT(o_final, ni & 1, kStatusMmaTimeout);
+            PP_WAIT(o_final, ni & 1);
             tc_fence_after();
             auto finish = [&](int d, float4 v, float inv) { // dims d .. d + 3 of this thread's row
                 v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
@@ -763,6 +760,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             }
         }
     }
+    goto done;
+failed:
+    if (lane == 0) atomicOr(a.words, kStatusMmaTimeout);
 done:
     if (warp == 20) { // what was issued lands before the shared memory goes (it has, unless a wait gave up)
         for (uint32_t k = copied_k > NK ? copied_k - NK : 0; k < copied_k; k++) mbar_wait(&k_full[k % NK], (k / NK) & 1, never_set, 200000u);
@@ -773,8 +773,6 @@ done:
     tc_fence_after();
     __syncwarp();
     if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-#undef PP_WAIT_FOR
-#undef PP_WAIT_AHEAD
 #undef PP_WAIT
 #undef PP_MEET_ALL
 }
