@@ -32,14 +32,33 @@ constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the va
 constexpr float kPpShift = 5.5f, kPpHalf = -8.f /* see split_weights */, kPpRescale = 3.f, kPpSpare = 0.5f;
 constexpr int kPpScaleRing = 4, kPpScales = 9;
 
+// What the roles of a CTA need of an item: one warp walks the items and leaves this in a small ring of shared memory.  (With a walk in
+// each role's registers they spilled, and of the 256 KB an SM has for L1 and shared memory this kernel leaves L1 so little that the spills
+// missed it: every step of every role took hundreds of clocks.)
+struct PpItem {
+    uint32_t kt0, kt1;      // key tiles; kt0 == kt1: no more items
+    int32_t lim0;           // keys that the first token sees
+    uint32_t seq, head;
+    uint32_t row0, ntok;    // first row of q, tokens
+    uint32_t keys;          // that the last token sees: those to be copied
+    uint32_t span;          // the CTAs it lies in: the first, and how many << 16
+    float vref;             // by which O is kept after the last tile (written with that tile's scales)
+};
+constexpr int kPpItems = 3;
+constexpr int kPpItemReaders = 2 /* products */ + 1 /* scales */ + 4 /* Q rows */ + kPpWarps;
+
 template <int D, int PARTS>
 struct PpLayout {
     static constexpr int kSlabs = D / 128;
     static constexpr int kQPart = kPpRows * D;
     static constexpr int kStage = kPpKeys * D; // K or V of a tile
-    static constexpr int kKStages = D == 256 ? (PARTS == 2 ? 3 : 2) : 4, kVStages = D == 256 ? 2 : 4;
+    static constexpr int kKStages = D == 256 ? 2 : 4, kVStages = D == 256 ? 2 : 4;
     static constexpr int kRing = (kKStages + kVStages) * kStage;
-    static constexpr int kSmem = PARTS * kQPart + kRing + 3072 /* statistics, scales, barriers */;
+    // the statistics' area: maxima, scales, items, the share, barriers, four words, the rows' exponents
+    static constexpr int kBarriers = 2 * (kKStages + kVStages) + 2 * kPpScaleRing + 2 * kPpItems + 3 * 2 + 6 + 16;
+    static constexpr int kStats = 4 * 2 * kPpRows * 2 + kPpScaleRing * kPpScales * 8 + kPpItems * int(sizeof(PpItem)) + int(sizeof(PagedShare)) + kBarriers * 8 + 16 + kPpRows;
+    static_assert((kPpItems * sizeof(PpItem)) % 8 == 0 && sizeof(PagedShare) % 8 == 0, "barriers stand at multiples of 8 bytes");
+    static constexpr int kSmem = PARTS * kQPart + kRing + kStats;
     // O; the scores of one tile; the weights' buffers, one or two
     static constexpr int kPBufs = D == 256 && PARTS == 3 ? 1 : 2;
     static constexpr int kPCols = 32 * PARTS;
@@ -194,21 +213,6 @@ __device__ __forceinline__ float lg2_approx(float x) {
     return y;
 }
 
-// What the roles of a CTA need of an item: one warp walks the items and leaves this in a small ring of shared memory.  (With a walk in
-// each role's registers they spilled, and of the 256 KB an SM has for L1 and shared memory this kernel leaves L1 so little that the spills
-// missed it: every step of every role took hundreds of clocks.)
-struct PpItem {
-    uint32_t kt0, kt1;      // key tiles; kt0 == kt1: no more items
-    int32_t lim0, vis;      // keys that the first and the last token see
-    uint32_t seq, head;
-    uint32_t row0, ntok;    // first row of q, tokens
-    uint32_t keys;          // to be copied
-    uint32_t c0, parts;     // the CTAs it lies in
-    uint32_t pad;
-};
-constexpr int kPpItems = 4;
-constexpr int kPpItemReaders = 2 /* products */ + 1 /* scales */ + 4 /* Q rows */ + kPpWarps;
-
 template <int D, int PARTS>
 __global__ void __launch_bounds__(kPpThreads, 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedArgs a, const uint32_t tpt) {
@@ -218,22 +222,22 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     uint8_t *sQ = smem;                                  // [part][slab][128 rows][128 dims]
     uint8_t *ring = sQ + PARTS * L::kQPart;              // [K stages, V stages][slab][128 keys][128 dims]
     uint8_t *ring_v = ring + NK * L::kStage;
-    // the statistics' area, 3 KB
-    __nv_bfloat16 *xch = reinterpret_cast<__nv_bfloat16 *>(ring + L::kRing); // [team][half][128 rows]: maxima, rounded up
-    float *lx = reinterpret_cast<float *>(xch);                              // at a tile's end: [2][128 rows] sums
-    __nv_bfloat16 *mpub = xch + 512;                                         // [2][128 rows]: the running maxima after a tile
-    float2 *scl = reinterpret_cast<float2 *>(mpub + 256);                    // [kPpScaleRing][8]: key scale (-1: bad block), log2 r; then
-                                                                             // what vref falls by against the tile before, vref
+    // the statistics' area
+    __nv_bfloat16 *xch = reinterpret_cast<__nv_bfloat16 *>(ring + L::kRing); // [4 tiles][2 halves][128 rows]: maxima, rounded up
+    float *lx = reinterpret_cast<float *>(xch);                              // at a tile's end: [4][128 rows] sums
+    float2 *scl = reinterpret_cast<float2 *>(xch + 1024);                    // [kPpScaleRing][8]: key scale (-1: bad block), log2 r; then
+                                                                             // what vref falls by against the tile before
     PpItem *items = reinterpret_cast<PpItem *>(scl + kPpScaleRing * kPpScales);
     PagedShare *share = reinterpret_cast<PagedShare *>(items + kPpItems);
     uint64_t *bars = reinterpret_cast<uint64_t *>(share + 1);
-    uint64_t *k_full = bars, *v_full = bars + 4, *k_empty = bars + 8, *v_empty = bars + 12, *sc_full = bars + 16, *sc_empty = bars + 20,
-             *item_full = bars + 24, *item_empty = bars + 28, *s_full = bars + 32 /* one for each team: a wait by parity must not find the other's phase */,
-             *p_full = bars + 34, *pv_done = bars + 36, *q_full = bars + 38, *q_empty = bars + 39, *s_free = bars + 40, *o_final = bars + 41,
-             *o_empty = bars + 42, *all_met = bars + 43, *pair_met = bars + 44 /* [team][row quarter] */, *m_full = bars + 52 /* [2][4 row quarters] */;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 60);
+    uint64_t *k_full = bars, *v_full = k_full + NK, *k_empty = v_full + NV, *v_empty = k_empty + NK, *sc_full = v_empty + NV, *sc_empty = sc_full + kPpScaleRing,
+             *item_full = sc_empty + kPpScaleRing, *item_empty = item_full + kPpItems,
+             *s_full = item_empty + kPpItems /* one for each team: a wait by parity must not find the other's phase */, *p_full = s_full + 2,
+             *pv_done = p_full + 2, *q_full = pv_done + 2, *q_empty = q_full + 1, *s_free = q_full + 2, *o_final = q_full + 3, *o_empty = q_full + 4,
+             *all_met = q_full + 5, *x_met = q_full + 6 /* [4 tiles][4 row quarters] */;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(x_met + 16);
     volatile uint32_t *never_set = tmem_slot + 1, *arrived = tmem_slot + 2;
-    uint8_t *row_e = reinterpret_cast<uint8_t *>(bars + 62); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
+    uint8_t *row_e = reinterpret_cast<uint8_t *>(tmem_slot + 4); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
 
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (smem_u32(smem) & 1023) { // the swizzle and the descriptors count on it
@@ -241,12 +245,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         return;
     }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 4; s++) {
-            mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1), mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
-            mbar_init(&sc_full[s], 1), mbar_init(&sc_empty[s], 1), mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], kPpItemReaders);
-        }
-        for (int s = 0; s < 2; s++) mbar_init(&s_full[s], 1), mbar_init(&p_full[s], kPpWarps / 2), mbar_init(&pv_done[s], 1);
-        for (int s = 0; s < 8; s++) mbar_init(&pair_met[s], 2), mbar_init(&m_full[s], 1);
+        for (int s = 0; s < NK; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
+        for (int s = 0; s < NV; s++) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
+        for (int s = 0; s < kPpScaleRing; s++) mbar_init(&sc_full[s], 1), mbar_init(&sc_empty[s], 1);
+        for (int s = 0; s < kPpItems; s++) mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], kPpItemReaders);
+        for (int s = 0; s < 2; s++) mbar_init(&s_full[s], 2), mbar_init(&p_full[s], kPpWarps / 2), mbar_init(&pv_done[s], 1);
+        for (int s = 0; s < 16; s++) mbar_init(&x_met[s], 2);
         mbar_init(q_full, 4), mbar_init(q_empty, 1 + kPpWarps), mbar_init(s_free, kPpWarps / 2), mbar_init(o_final, 1), mbar_init(o_empty, kPpWarps);
         mbar_init(all_met, kPpWarps);
         *never_set = 0;
@@ -298,7 +302,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         kk = it.kt0, kk1 = it.kt1, keys = walk.tiles.keys(it.q, it.rtile), head = it.head;
                         table = a.tables + size_t(it.seq) * a.table_stride;
                         if (lane == 0) {
-                            items[ni % kPpItems] = PpItem{it.kt0, it.kt1, it.lim0, paged_visible(it), it.seq, it.head, it.q.row0 + it.tok0, it.ntok, keys, span.x, span.y, 0};
+                            items[ni % kPpItems] = PpItem{it.kt0, it.kt1, it.lim0, it.seq, it.head, it.q.row0 + it.tok0, it.ntok, keys, span.x | span.y << 16, 0.f};
                             mbar_arrive(&item_full[ni % kPpItems]);
                         }
                         __syncwarp();
@@ -350,7 +354,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 for (; g < end; g++) {
                     const uint32_t st = g % NK;
                     PP_WAIT(&k_full[st], g / NK & 1);
+                    PP_WAIT(&sc_full[g % kPpScaleRing], g / kPpScaleRing & 1);
                     PP_WAIT(s_free, (g & 1) ^ 1);
+                    if (lane == 0) mbar_arrive(&s_full[g & 1]); // hands the tile's scales on; the scores follow
                     tc_fence_after();
                     __syncwarp();
                     const uint32_t bd = bd0 + st * (L::kStage >> 4);
@@ -374,8 +380,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 uint32_t kt = it.kt0;
                 const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
                 if (kt == kt1) break;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
                 float vref = 0.f;
                 for (; kt < kt1; kt++, g++) {
                     const uint32_t ss = g % kPpScaleRing, key = kt * kPpKeys + lane * 16;
@@ -401,9 +405,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     vref = top;
                     PP_WAIT(&sc_empty[ss], (g / kPpScaleRing & 1) ^ 1);
                     if (lane < kPpScales) scl[ss * kPpScales + lane] = v;
+                    if (lane == 0 && kt + 1 == kt1) items[ni % kPpItems].vref = vref;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[ss]);
                 }
+                if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
             }
         } else {
             // ------------------------------------------------------------ value products
@@ -412,7 +418,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             uint32_t g = 0;
             for (uint32_t ni = 0;; ni++) {
                 PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
-                const int32_t vis = items[ni % kPpItems].vis;
+                const int32_t keys = int32_t(items[ni % kPpItems].keys);
                 const uint32_t kt0 = uniform(items[ni % kPpItems].kt0), kt1 = uniform(items[ni % kPpItems].kt1);
                 if (kt0 == kt1) break;
                 __syncwarp();
@@ -424,10 +430,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     // rows behind the last key, and of bad blocks, may hold NaN, which a weight of 0 does not silence
                     const int32_t key0 = int32_t(kt * kPpKeys);
                     const uint32_t bad = __ballot_sync(0xffffffffu, lane < 8 && scl[ss * kPpScales + (lane & 7)].x < 0.f);
-                    if (key0 + kPpKeys > vis || bad) {
+                    if (key0 + kPpKeys > keys || bad) {
                         for (uint32_t k = lane; k < kPpKeys * 8 * kSlabs; k += 32) {
                             const uint32_t key = (k >> 3) % kPpKeys, slab = k / (kPpKeys * 8);
-                            if (key0 + int32_t(key) >= vis || (bad >> (key >> 4) & 1))
+                            if (key0 + int32_t(key) >= keys || (bad >> (key >> 4) & 1))
                                 *reinterpret_cast<uint4 *>(ring_v + st * L::kStage + slab * (kPpKeys * 128) + key * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
                         fence_async_smem();
@@ -512,7 +518,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         // tensor memory, the weights written over them: 1.94, the two teams in step and the products between them.)
         const uint32_t quarter = warp & 3, half = warp >> 2 & 1, team = warp >> 3, row = quarter * 32 + lane;
         const uint32_t lane_addr = (quarter * 32) << 16;
-        uint32_t g = 0, met = 0, all = 0; // tiles, meetings of the pair, of all warps, so far
+        uint32_t g = 0, all = 0; // tiles, meetings of all warps, so far
         for (uint32_t ni = 0;; ni++) {
             PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
             const uint32_t kt0 = items[ni % kPpItems].kt0, kt1 = items[ni % kPpItems].kt1;
@@ -523,12 +529,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const float rs = __uint_as_float(uint32_t(row_e[row]) << 23) * a.scale_log2;
             __syncwarp();
             if (lane == 0) mbar_arrive(q_empty); // the factor has been read
-            float m = -INFINITY, l = 0.f; // the maximum that l goes by
+            float m = -INFINITY, l = 0.f;
+            // The running maximum after a tile whose own is `top` (the same in all four warps that share the rows).
+            auto follow = [&](float was, float top) {
+                const bool need = __any_sync(0xffffffffu, top > was + kPpRescale);
+                return need ? fmaxf(was, __bfloat162float(__float2bfloat16_ru(top + kPpSpare))) : was;
+            };
             for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
                 if ((g & 1) != team) continue;
                 const int32_t key0 = int32_t(kt * kPpKeys + half * 64);
                 const uint32_t ss = g % kPpScaleRing, pb = g % NP;
-                PP_WAIT(&sc_full[ss], g / kPpScaleRing & 1);
                 const float2 *sc = scl + ss * kPpScales + half * 4;
                 PP_WAIT(&s_full[team], g >> 1 & 1);
                 tc_fence_after();
@@ -556,31 +566,27 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     t[0] = max3(t[0], x[6], x[7]), t[1] = max3(t[1], x[8], x[9]), t[0] = max3(t[0], x[10], x[11]), t[1] = max3(t[1], x[12], x[13]);
                     mx = fmaxf(mx, fmaxf(max3(t[0], x[14], x[15]), t[1]) * (fabsf(f) * rs));
                 }
-                // the two threads of a row agree on one maximum (rounded up it is still one that no score passes), and with the other
-                // team's of the tile before
-                __nv_bfloat16 *x = xch + team * 256;
-                x[half * 128 + row] = __float2bfloat16_ru(mx);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&pair_met[team * 4 + quarter]);
+                // The two threads of a row agree on one maximum (rounded up it is still one that no score passes).  Every warp follows the running
+                // maximum through all tiles: the other team's tile first, then its own.  (Waiting for the other team's tile also shows
+                // that its slot of four tiles ago has been read.)
+                const uint32_t xs = g & 3;
                 float m_was = -INFINITY;
                 if (kt > kt0) {
-                    PP_WAIT(&m_full[((g - 1) & 1) * 4 + quarter], (g - 1) >> 1 & 1);
-                    m_was = __bfloat162float(mpub[((g - 1) & 1) * 128 + row]);
+                    const uint32_t xo = (g - 1) & 3;
+                    PP_WAIT(&x_met[xo * 4 + quarter], (g - 1) >> 2 & 1);
+                    m_was = follow(m, fmaxf(__bfloat162float(xch[xo * 256 + row]), __bfloat162float(xch[xo * 256 + 128 + row])));
                 }
-                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1);
-                const float top = fmaxf(__bfloat162float(x[row]), __bfloat162float(x[128 + row]));
-                const bool need = __any_sync(0xffffffffu, top > m_was + kPpRescale);
-                const float mt = need ? fmaxf(m_was, __bfloat162float(__float2bfloat16_ru(top + kPpSpare))) : m_was;
-                if (half == 0) mpub[(g & 1) * 128 + row] = __float2bfloat16(mt);
+                const __nv_bfloat16 up = __float2bfloat16_ru(mx);
+                xch[xs * 256 + half * 128 + row] = up;
                 __syncwarp();
-                if (lane == 0) {
-                    if (half == 0) mbar_arrive(&m_full[(g & 1) * 4 + quarter]);
-                    mbar_arrive(&pair_met[team * 4 + quarter]); // this tile's maxima have been read
-                }
-                if (mt != m) { // (also where the other team has moved it)
+                if (lane == 0) mbar_arrive(&x_met[xs * 4 + quarter]);
+                PP_WAIT(&x_met[xs * 4 + quarter], g >> 2 & 1);
+                const float mt = follow(m_was, fmaxf(__bfloat162float(up), __bfloat162float(xch[xs * 256 + (half ^ 1) * 128 + row])));
+                if (mt != m) {
                     l *= ex2_approx(m - mt); // 0 for the first
                     m = mt;
                 }
+                const bool need = __any_sync(0xffffffffu, mt != m_was);
                 const float fv = scl[ss * kPpScales + 8].x;
                 if (kt > kt0 && (need || fv != 1.f)) {
                     // The product of the tile before must have landed in O.  (That of two tiles before first: it shares no barrier with it, and
@@ -643,34 +649,29 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[pb]);
-                PP_WAIT(&pair_met[team * 4 + quarter], met++ & 1); // (long over)
             }
             // ---- the tile's end: the four sums of a row become one, O leaves tensor memory
 #define PP_MEET_ALL()                                      \
     __syncwarp();                                          \
     if (lane == 0) mbar_arrive(all_met);                   \
     PP_WAIT(all_met, all++ & 1)
-            PP_MEET_ALL(); // the last tile's maximum is there; the exchange area is free for the sums
-            const float vref = scl[((g - 1) % kPpScaleRing) * kPpScales + 8].y;
-            {
-                const float mt = __bfloat162float(mpub[((g - 1) & 1) * 128 + row]);
+            if (((g - 1) & 1) != team) { // the last tile was the other team's
+                PP_WAIT(&x_met[((g - 1) & 3) * 4 + quarter], (g - 1) >> 2 & 1);
+                const float mt = follow(m, fmaxf(__bfloat162float(xch[((g - 1) & 3) * 256 + row]), __bfloat162float(xch[((g - 1) & 3) * 256 + 128 + row])));
                 if (mt != m) l *= ex2_approx(m - mt);
                 m = mt;
             }
-            if (half) lx[team * 128 + row] = l;
+            PP_MEET_ALL(); // all maxima have been read: the sums take their place
+            lx[(team * 2 + half) * 128 + row] = l;
             PP_MEET_ALL();
-            if (!half) l += lx[team * 128 + row];
-            PP_MEET_ALL();
-            if (!half) lx[team * 128 + row] = l;
-            PP_MEET_ALL();
-            l = (lx[row] + lx[128 + row]) * 256.f; // (the weights' sums were taken times 2^-8)
+            l = ((lx[row] + lx[128 + row]) + (lx[256 + row] + lx[384 + row])) * 256.f; // (the weights' sums were taken times 2^-8)
             PP_MEET_ALL();
             const PpItem &it = items[ni % kPpItems];
             const uint32_t cq = warp >> 2, tok = row / a.group, hq = row % a.group;
             const bool live = tok < it.ntok && row < tpt * a.group;
-            const uint32_t parts = it.parts;
+            const uint32_t c0 = it.span & 0xffff, parts = it.span >> 16;
             const size_t orow = live ? size_t(it.row0 + tok) * a.heads + it.head * a.group + hq : 0;
-            const uint32_t c0 = it.c0;
+            const float vref = it.vref;
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
             PP_WAIT(o_final, ni & 1);
