@@ -487,7 +487,7 @@ int saetta_paged_attention_create(int device, size_t heads, size_t kv_heads, siz
     op->ctas = sm_count(device);
     op->part_floats = 128 * (head_dim + 2) + 4; // 128 rows: the largest tile; (m, l) of each; the value scale O is kept by
     void *p = nullptr, *w = nullptr;
-    const size_t words = size_t(kPagedCounters) + 2 * size_t(op->ctas);
+    const size_t words = size_t(kPagedCounters) + 3 * size_t(op->ctas);
     cudaError_t e = cudaMalloc(&p, size_t(op->ctas) * 2 * op->part_floats * sizeof(float));
     op->parts = static_cast<float *>(p);
     if (e == cudaSuccess) e = cudaMalloc(&w, words * sizeof(uint32_t));
@@ -538,7 +538,7 @@ int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *ca
     a.q_dtype = q_dtype, a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
     // which kernel: see kPagedFewRows
-    if (batch.max_rows * a.group <= kPagedFewRows) return launch_paged_decode(a, cache, op->ctas, cudaStream_t(stream));
+    if (batch.max_rows * a.group <= kPagedFewRows) return launch_paged_decode(a, cache, uint32_t(batch.max_rows * a.group), op->ctas, cudaStream_t(stream));
     return launch_paged_prefill(a, cache, op->ctas, cudaStream_t(stream));
 }
 

@@ -29,7 +29,7 @@ constexpr int kPagedBadScale = 2;         // word index of the (-1, -1) pair
 constexpr int kPagedCounters = 8;
 constexpr int kPagedMaxGroup = 16;        // query heads of one kv head
 constexpr size_t kPagedMaxSeqs = 8192;
-constexpr size_t kPagedFewRows = 32;      // rows (tokens x heads of a kv head) of a sequence up to which the few-rows kernel runs
+constexpr size_t kPagedFewRows = 16;      // rows (tokens x heads of a kv head) of a sequence up to which the few-rows kernel runs
 
 // What an attention launch reads and writes.
 struct PagedArgs {
@@ -49,7 +49,7 @@ struct PagedArgs {
     float scale_log2;
 };
 
-int launch_paged_decode(const PagedArgs &a, const saetta_paged_cache *cache, int ctas, cudaStream_t stream);
+int launch_paged_decode(const PagedArgs &a, const saetta_paged_cache *cache, uint32_t rows, int ctas, cudaStream_t stream); // rows of a sequence x its heads per kv head, at most
 int paged_decode_configure(int device);
 int launch_paged_prefill(const PagedArgs &a, const saetta_paged_cache *cache, int ctas, cudaStream_t stream);
 int paged_prefill_configure(int device);

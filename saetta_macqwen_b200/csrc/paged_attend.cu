@@ -7,9 +7,9 @@
 // kv head; the rest is arranged so that these stream without a pause:
 //
 //  * One CTA for each SM takes an equal share of all key tiles (paged_sched.cuh); a producer warp keeps a ring of
-//    64-key tiles of K and V in flight (TMA tensor copies of whole pages, 128-byte swizzle: 160 KB on the way with
-//    head dim 256) and the pages' scales beside them (8-byte asynchronous copies).
-//  * Eight consumer warps, four for each tile, 16 keys a warp, each with its own running maximum, sum and accumulators: no
+//    tiles of K and V in flight (64 keys with head dim 256, 128 with 128; TMA tensor copies of whole pages, 128-byte
+//    swizzle: 160 KB on the way) and the pages' scales beside them (8-byte asynchronous copies).
+//  * Eight consumer warps, four for each tile, 16 or 32 keys a warp, each with its own running maximum, sum and accumulators: no
 //    barrier between tiles.  Keys are the 16 rows of mma.m16n8k16, query rows its 8 columns (a group of 8 heads fills them).
 //    The order of dims inside a product is free, so a lane feeds 16 consecutive bytes of a key to four products; with the
 //    swizzle, chunk 2 t + j for lane t of a key makes these 128-bit loads free of bank conflicts, and chunk g for lane
@@ -25,20 +25,23 @@
 
 namespace saetta {
 
-constexpr int kPdTile = 64;      // keys of a tile
-constexpr int kPdThreads = 288;  // 8 consumer warps, 1 producer warp
+constexpr int kPdThreads = 384;  // 8 consumer warps, the producer's group of 4 (one of them works)
+constexpr uint32_t kPdGroup = 12; // parts of an item that one CTA joins by itself
 constexpr float kPdRescale = 8.f; // the accumulators follow the running maximum only past this many doublings
 
 template <int D, int NT>
 struct PdLayout {
     static constexpr int kRows = 8 * NT;
-    static constexpr int kSide = kPdTile * D;
-    static constexpr int kStage = 2 * kSide;
-    static constexpr int kStages = D == 256 ? 5 : 8;
+    static constexpr int kSub = D == 256 ? 1 : 2;  // 16-key pieces that a warp takes of a tile
+    static constexpr int kTile = 64 * kSub;        // keys of a tile
+    static constexpr int kSide = kTile * D;
+    static constexpr int kStage = 2 * kSide;       // 32 KB
+    static constexpr int kStages = 5;
+    static constexpr int kPages = kTile / 16;      // of a tile, at most
     static constexpr int kRow = 128 + 4;                      // floats of one row of the exchange buffer
     static constexpr int kExchange = 8 * 8 * kRow * 4;        // 8 warps x 8 rows of 128 dims
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * 4 * 8 /*scales*/ + 3072 /*barriers, statistics*/;
+    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * kPages * 8 /*scales*/ + 3072 /*barriers, statistics*/;
 };
 static_assert(PdLayout<256, 2>::kSmem <= 227 * 1024 && PdLayout<128, 2>::kSmem <= 227 * 1024, "fits a CTA's shared memory");
 
@@ -47,6 +50,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(w)));
     return h;
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void cp_async8(void *dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
@@ -65,12 +69,12 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kPdThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedArgs a, const uint32_t tpt) {
     using L = PdLayout<D, NT>;
-    constexpr int kSlabs = D / 128, R = L::kRows;
+    constexpr int kSlabs = D / 128, R = L::kRows, kTile = L::kTile, U = L::kSub;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *xch = reinterpret_cast<float *>(ring + L::kRing);                  // [8 warps][8 rows][kRow]
-    float2 *scl = reinterpret_cast<float2 *>(ring + L::kRing + L::kExchange); // [stage][4 pages]
-    uint64_t *full = reinterpret_cast<uint64_t *>(scl + L::kStages * 4), *empty = full + L::kStages;
+    float2 *scl = reinterpret_cast<float2 *>(ring + L::kRing + L::kExchange); // [stage][page]
+    uint64_t *full = reinterpret_cast<uint64_t *>(scl + L::kStages * L::kPages), *empty = full + L::kStages;
     uint64_t *scratch = empty + L::kStages; // 40 words
     PagedShare *share = reinterpret_cast<PagedShare *>(scratch + 40);
     float *wm = reinterpret_cast<float *>(share + 1); // [8][R] maxima, then sums, then weights; [R] joint maximum and sum
@@ -85,28 +89,32 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         *abort_flag = 0, *never_set = 0;
         mbar_fence_init();
     }
+    if (tid == kPdThreads - 1) prefetch_map(&map_k), prefetch_map(&map_v);
     pdl_wait();
-    paged_share<kPdTile>(a, tpt, kPdThreads, 1, scratch, share);
+    paged_share<kTile>(a, tpt, kPdThreads, 1, scratch, share);
     if (share->x0 >= share->x1) return;
     auto give_up = [&](uint32_t bit) {
         atomicOr(a.words, bit);
         *abort_flag = 1;
     };
-    const uint32_t bt = min(a.block_tokens, uint32_t(kPdTile)); // keys of one copy
+    const uint32_t bt = min(a.block_tokens, uint32_t(kTile)); // keys of one copy
     const uint32_t G = a.group;
-    PagedWalk<kPdTile> walk(a, *share, tpt);
+    PagedWalk<kTile> walk(a, *share, tpt);
     PagedItem it;
 
-    if (warp == 8) {
+    // registers: 256 x 232 + 128 x 40 = the 384 x 168 of the launch
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp > 8) return;
         // ------------------------------------------------------------ producer
         uint32_t g = 0;
         bool ok = true;
         while (ok && walk.next(it)) {
             const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
             const uint32_t keys = walk.tiles.keys(it.q, it.rtile);
-            const uint32_t per_tile = kPdTile / bt;
+            const uint32_t per_tile = kTile / bt;
             auto block_of = [&](uint32_t kt) -> int32_t { // of this lane's page of a tile; -2: none
-                const uint32_t key = kt * kPdTile + lane * bt;
+                const uint32_t key = kt * kTile + lane * bt;
                 return lane < per_tile && key < keys ? table[key / a.block_tokens] : -2;
             };
             int32_t next = block_of(it.kt0);
@@ -123,13 +131,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 __syncwarp();
                 if (good) {
                     uint8_t *dst = ring + st * L::kStage + lane * bt * D;
-                    const uint32_t key = kt * kPdTile + lane * bt;
+                    const uint32_t key = kt * kTile + lane * bt;
                     const int row = int((uint32_t(block) * a.kv_heads + it.head) * a.block_tokens + (key & (a.block_tokens - 1)));
                     tma_load_3d(dst, &map_k, &full[st], 0, row, 0);
                     tma_load_3d(dst + L::kSide, &map_v, &full[st], 0, row, 0);
                 }
                 if (want) // a bad block's keys are marked by its scales
-                    cp_async8(&scl[st * 4 + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
+                    cp_async8(&scl[st * L::kPages + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
                                                         : reinterpret_cast<const float *>(a.words + kPagedBadScale));
                 cp_async_arrive(&full[st]);
             }
@@ -140,6 +148,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         return;
     }
 
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ------------------------------------------------------------ consumers
     const uint32_t gi = lane >> 2, t = lane & 3, sub = warp & 3, team = warp >> 2;
     uint32_t g = 0;
@@ -203,19 +212,34 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
             if (ok && !mbar_wait(&full[st], ph, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
             if (!ok) continue;
-            const int32_t key0 = int32_t(kt * kPdTile + sub * 16);
-            const uint32_t page = sub * 16 / bt, in = sub * 16 % bt;
-            const float2 sc = scl[st * 4 + page];
-            if (key0 < vis && sc.x >= 0.f) {
-                const uint32_t kbase = smem_u32(ring) + st * L::kStage + page * bt * D;
-                float s[NT][4];
+            const int32_t key0 = int32_t(kt * kTile + sub * 16 * U);
+            if (key0 < vis) {
+                uint32_t kbase[U], in[U];
+                float2 sc[U];
+                bool use[U];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+                for (int u = 0; u < U; u++) {
+                    const uint32_t at = (sub * U + u) * 16, page = at / bt;
+                    in[u] = at % bt;
+                    kbase[u] = smem_u32(ring) + st * L::kStage + page * bt * D;
+                    sc[u] = scl[st * L::kPages + page];
+                    use[u] = key0 + u * 16 < vis && sc[u].x >= 0.f; // not behind the last key, not of a bad block
+                    if (!use[u]) sc[u] = make_float2(1.f, 0.f);
+                }
+                // four chains of products: one after the other they would wait for one another
+                constexpr int kChains = kSlabs * 2;
+                float acc[U][kChains][NT][4];
 #pragma unroll
-                for (int sl = 0; sl < kSlabs; sl++)
+                for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t row = in + gi, at = kbase + sl * bt * 128 + row * 128 + (((2 * t + j) ^ (row & 7)) << 4);
+                    for (int c = 0; c < kChains; c++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) acc[u][c][nt][0] = acc[u][c][nt][1] = acc[u][c][nt][2] = acc[u][c][nt][3] = 0.f;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int c = 0; c < kChains; c++) {
+                        const uint32_t row = in[u] + gi, at = kbase[u] + (c >> 1) * bt * 128 + row * 128 + (((2 * t + (c & 1)) ^ (row & 7)) << 4);
                         const uint4 lo = lds128(at), hi = lds128(at + 8 * 128); // key gi, key gi + 8 (the same swizzle)
                         const uint32_t wl4[4] = {lo.x, lo.y, lo.z, lo.w}, wh4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -223,25 +247,36 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             const uint32_t a0 = e4m3x2_to_h2(wl4[e]), a1 = e4m3x2_to_h2(wh4[e]);
                             const uint32_t a2 = e4m3x2_to_h2(wl4[e] >> 16), a3 = e4m3x2_to_h2(wh4[e] >> 16);
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) mma_f16(s[nt], a0, a1, a2, a3, qf[nt][sl * 8 + j * 4 + e][0], qf[nt][sl * 8 + j * 4 + e][1]);
+                            for (int nt = 0; nt < NT; nt++) mma_f16(acc[u][c][nt], a0, a1, a2, a3, qf[nt][c * 4 + e][0], qf[nt][c * 4 + e][1]);
                         }
                     }
-                const bool edge = key0 + 16 > it.lim0;
-                const float vnew = fmaxf(vref, sc.y);
-                uint32_t pb[NT][2];
+                const bool edge = key0 + 16 * U > it.lim0;
+                float vnew = vref;
+                bool all_used = true;
+#pragma unroll
+                for (int u = 0; u < U; u++) vnew = fmaxf(vnew, sc[u].y), all_used &= use[u];
+                float s[U][NT][4];
+                uint32_t pb[U][NT][2];
                 bool need = vnew != vref;
                 float f[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const float c = sc.x * rs[nt][j];
-                        s[nt][j] *= c, s[nt][2 + j] *= c;
-                        if (edge) {
-                            if (key0 + int32_t(gi) >= lim[nt][j]) s[nt][j] = -INFINITY;
-                            if (key0 + int32_t(gi) + 8 >= lim[nt][j]) s[nt][2 + j] = -INFINITY;
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
+                            const float c = sc[u].x * rs[nt][j];
+#pragma unroll
+                            for (int k = 0; k < 2; k++) { // key gi, key gi + 8
+                                float x = acc[u][0][nt][2 * k + j] + acc[u][1][nt][2 * k + j];
+                                if (kChains == 4) x += acc[u][kChains - 2][nt][2 * k + j] + acc[u][kChains - 1][nt][2 * k + j];
+                                x *= c;
+                                if ((edge && key0 + u * 16 + int32_t(gi) + 8 * k >= lim[nt][j]) || !use[u]) x = -INFINITY;
+                                s[u][nt][2 * k + j] = x;
+                                mx = fmaxf(mx, x);
+                            }
                         }
-                        float mx = fmaxf(s[nt][j], s[nt][2 + j]);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -265,41 +300,46 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         }
                     vref = vnew;
                 }
-                const float vr = vref > 0.f ? sc.y / vref : 0.f;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float p[4];
+                for (int u = 0; u < U; u++) {
+                    const float vr = vref > 0.f ? sc[u].y / vref : 0.f;
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-                        p[j] = ex2_approx(s[nt][j] - mu), p[2 + j] = ex2_approx(s[nt][2 + j] - mu);
-                        l[nt][j] += p[j] + p[2 + j];
-                    }
-                    pb[nt][0] = movmatrix_trans(pack_half2(p[0] * vr, p[1] * vr));
-                    pb[nt][1] = movmatrix_trans(pack_half2(p[2] * vr, p[3] * vr));
-                }
-                const bool tail = key0 + 16 > vis; // what lies behind the last key is any byte, NaN too: no product may read it
+                    for (int nt = 0; nt < NT; nt++) {
+                        float p[4];
 #pragma unroll
-                for (int sl = 0; sl < kSlabs; sl++) {
-                    uint4 v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t key = 2 * t + (k & 1) + (k >> 1) * 8, row = in + key;
-                        v[k] = lds128(kbase + L::kSide + sl * bt * 128 + row * 128 + ((gi ^ (row & 7)) << 4));
-                        if (tail && key0 + int32_t(key) >= vis) v[k] = make_uint4(0, 0, 0, 0);
-                    }
-                    const uint32_t w[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
-                                              {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t x = prmt(w[0][e], w[1][e], h ? 0x7362 : 0x5140), y = prmt(w[2][e], w[3][e], h ? 0x7362 : 0x5140);
-                            const uint32_t a0 = e4m3x2_to_h2(x), a1 = e4m3x2_to_h2(x >> 16), a2 = e4m3x2_to_h2(y), a3 = e4m3x2_to_h2(y >> 16);
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][sl * 8 + e * 2 + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        for (int j = 0; j < 2; j++) {
+                            const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+                            p[j] = ex2_approx(s[u][nt][j] - mu), p[2 + j] = ex2_approx(s[u][nt][2 + j] - mu);
+                            l[nt][j] += p[j] + p[2 + j];
                         }
+                        pb[u][nt][0] = movmatrix_trans(pack_half2(p[0] * vr, p[1] * vr));
+                        pb[u][nt][1] = movmatrix_trans(pack_half2(p[2] * vr, p[3] * vr));
+                    }
                 }
+                const bool tail = key0 + 16 * U > vis || !all_used; // what lies behind the last key is any byte, NaN too: no product may read it
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int sl = 0; sl < kSlabs; sl++) {
+                        uint4 v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t key = 2 * t + (k & 1) + (k >> 1) * 8, row = in[u] + key;
+                            v[k] = lds128(kbase[u] + L::kSide + sl * bt * 128 + row * 128 + ((gi ^ (row & 7)) << 4));
+                            if (tail && (key0 + u * 16 + int32_t(key) >= vis || !use[u])) v[k] = make_uint4(0, 0, 0, 0);
+                        }
+                        const uint32_t w[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                                  {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint32_t x = prmt(w[0][e], w[1][e], h ? 0x7362 : 0x5140), y = prmt(w[2][e], w[3][e], h ? 0x7362 : 0x5140);
+                                const uint32_t a0 = e4m3x2_to_h2(x), a1 = e4m3x2_to_h2(x >> 16), a2 = e4m3x2_to_h2(y), a3 = e4m3x2_to_h2(y >> 16);
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][sl * 8 + e * 2 + h], a0, a1, a2, a3, pb[u][nt][0], pb[u][nt][1]);
+                            }
+                    }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
@@ -374,46 +414,70 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (!whole) {
             float *ml = part + R * D;
             if (tid < R) ml[tid * 2] = rm[tid], ml[tid * 2 + 1] = rl[tid];
-            // the last CTA of the item to arrive joins the parts, in the order of the CTAs
+            // The parts are joined by the last CTA to arrive, in the order of the CTAs; many of them in two rounds, groups of some first, because one CTA
+            // reads no more than some 100 bytes a clock.
             const uint2 span = paged_ctas_of(*share, it);
             const uint32_t c0 = span.x, parts = span.y;
-            uint32_t *counter = a.words + kPagedCounters + c0;
-            __threadfence();
-            consumers_sync();
-            if (tid == 0) {
-                const uint32_t n = atomicAdd(counter, 1);
-                if (n + 1 == parts) *counter = 0;
-                *arrived = n + 1;
+            uint32_t per = parts; // parts of a group
+            if (parts > kPdGroup) {
+                per = 2;
+                while (per * per < parts) per++;
             }
-            consumers_sync();
-            if (*arrived == parts) {
-                __threadfence();
-                auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
-                float *wgt = xch; // [parts][R]
+            const uint32_t groups = (parts + per - 1) / per, mine = (blockIdx.x - c0) / per;
+            auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
+            // joins parts lo, lo + step, ... (n of them): into part lo, or the output
+            auto join = [&](uint32_t lo, uint32_t step, uint32_t n, bool last) {
+                float2 *in = reinterpret_cast<float2 *>(xch); // [n][R] maxima and sums; the maxima become weights
+                for (uint32_t i = tid; i < n * R; i += 256) in[i] = __ldcg(reinterpret_cast<const float2 *>(part_of(lo + i / R * step) + R * D) + i % R);
+                consumers_sync();
+                float top = -INFINITY, sum = 0.f;
                 if (tid < R) {
-                    float top = -INFINITY, sum = 0.f;
-                    for (uint32_t p = 0; p < parts; p++) top = fmaxf(top, __ldcg(part_of(p) + R * D + tid * 2));
+                    for (uint32_t p = 0; p < n; p++) top = fmaxf(top, in[p * R + tid].x);
                     const float mu = top == -INFINITY ? 0.f : top;
-                    for (uint32_t p = 0; p < parts; p++) {
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(part_of(p) + R * D + tid * 2));
+                    for (uint32_t p = 0; p < n; p++) {
+                        const float2 x = in[p * R + tid];
                         const float w = ex2_approx(x.x - mu);
-                        wgt[p * R + tid] = w;
+                        in[p * R + tid].x = w;
                         sum += x.y * w;
                     }
                     rl[tid] = sum;
                 }
                 consumers_sync();
+#pragma unroll 1
                 for (uint32_t i = tid; i < R * D / 4; i += 256) {
                     const uint32_t row = i * 4 / D, d = i * 4 % D;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-                    for (uint32_t p = 0; p < parts; p++) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(p) + row * D + d));
-                        const float wt = wgt[p * R + row];
+                    for (uint32_t p = 0; p < n; p++) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(lo + p * step) + row * D + d));
+                        const float wt = in[p * R + row].x;
                         v.x = fmaf(x.x, wt, v.x), v.y = fmaf(x.y, wt, v.y), v.z = fmaf(x.z, wt, v.z), v.w = fmaf(x.w, wt, v.w);
                     }
-                    finish(row, d, v, rl[row]);
+                    if (last) finish(row, d, v, rl[row]);
+                    else *reinterpret_cast<float4 *>(part_of(lo) + row * D + d) = v;
                 }
+                if (!last && tid < R) *reinterpret_cast<float2 *>(part_of(lo) + R * D + tid * 2) = make_float2(top, sum);
+            };
+            // whether this CTA is the last of `n` to come to the counter, which it then sets back
+            auto last_of = [&](uint32_t *counter, uint32_t n) {
+                __threadfence();
+                consumers_sync();
+                if (tid == 0) {
+                    const uint32_t k = atomicAdd(counter, 1) + 1;
+                    if (k == n) *counter = 0;
+                    *arrived = k;
+                }
+                consumers_sync();
+                const bool yes = *arrived == n;
+                if (yes) __threadfence();
+                consumers_sync();
+                return yes;
+            };
+            uint32_t *counters = a.words + kPagedCounters;
+            // a group's counter: by its first CTA, which may begin another item's tail as well
+            if (last_of(counters + (mine ? gridDim.x : 0) + c0 + mine * per, min(per, parts - mine * per))) {
+                join(mine * per, 1, min(per, parts - mine * per), groups == 1);
+                if (groups > 1 && last_of(counters + 2 * gridDim.x + c0, groups)) join(0, per, groups, true);
             }
         }
         consumers_sync(); // statistics and exchange buffer are free for the next item
@@ -434,12 +498,12 @@ int paged_decode_configure(int) {
     return rc;
 }
 
-int launch_paged_decode(const PagedArgs &a, const saetta_paged_cache *cache, int ctas, cudaStream_t stream) {
+int launch_paged_decode(const PagedArgs &a, const saetta_paged_cache *cache, uint32_t rows, int ctas, cudaStream_t stream) {
     CUtensorMap mk, mv;
-    const uint32_t box = std::min<uint32_t>(a.block_tokens, kPdTile), slabs = uint32_t(cache->head_dim / 128);
+    const uint32_t box = std::min<uint32_t>(a.block_tokens, cache->head_dim == 256 ? PdLayout<256, 1>::kTile : PdLayout<128, 1>::kTile), slabs = uint32_t(cache->head_dim / 128);
     if (int rc = paged_map(&mk, cache->keys, cache, box, slabs)) return rc;
     if (int rc = paged_map(&mv, cache->values, cache, box, slabs)) return rc;
-    const bool two = a.group > 8;
+    const bool two = rows > 8; // a product's columns hold 8 rows; two products for each piece of keys rather than two passes over the keys
     const uint32_t tpt = (two ? 16 : 8) / a.group; // tokens whose heads fill the product's columns
     void (*kernel)(CUtensorMap, CUtensorMap, PagedArgs, uint32_t) = nullptr;
     size_t smem = 0;

@@ -74,8 +74,18 @@ struct PagedShare {
     uint64_t total, x0, x1; // tiles of the launch, this CTA's
     uint64_t head_base;     // flat index of (seq, head 0, row tile 0)
     uint32_t ctas;          // that have a share
-    uint32_t seq, head, rtile;
+    uint32_t seq, head, rtile, kt0; // where it begins
+    PagedSeq q;             // of `seq`
 };
+
+// The CTAs that get a share: none of them less than min_tiles.
+__device__ __forceinline__ uint32_t paged_ctas(uint64_t total, uint32_t min_tiles) {
+    return uint32_t(min(uint64_t(gridDim.x), max(uint64_t(1), total >> 32 ? total / min_tiles : uint64_t((uint32_t(total) + min_tiles - 1) / min_tiles))));
+}
+// total * c / n for a CTA number c <= n < 256: in 32 bits where that holds (a division of 64-bit numbers takes some 500 clocks).
+__device__ __forceinline__ uint64_t paged_cut(uint64_t total, uint32_t c, uint32_t n) {
+    return total < (1u << 24) ? uint32_t(total) * c / n : total * c / n;
+}
 
 // Walks the items of a share; every role of a CTA walks the same ones.
 template <int T>
@@ -87,12 +97,8 @@ struct PagedWalk {
     PagedSeq q;
 
     __device__ __forceinline__ PagedWalk(const PagedArgs &args, const PagedShare &s, uint32_t tpt) : a(args), tiles{tpt} {
-        at = 0, end = uint32_t(s.x1 - s.x0), seq = s.seq, head = s.head, rtile = s.rtile, kt0 = 0, rtiles = 0;
-        if (end) {
-            q = paged_seq(a, seq);
-            rtiles = tiles.row_tiles(q);
-            kt0 = uint32_t(s.x0 - (s.head_base + uint64_t(head) * tiles.per_head(q) + tiles.before(q, rtile)));
-        }
+        at = 0, end = uint32_t(s.x1 - s.x0), seq = s.seq, head = s.head, rtile = s.rtile, kt0 = s.kt0, q = s.q;
+        rtiles = tiles.row_tiles(q);
     }
     __device__ __forceinline__ bool next(PagedItem &it) {
         if (at >= end) return false;
@@ -124,10 +130,10 @@ __device__ __forceinline__ int32_t paged_visible(const PagedItem &it) { return m
 
 // The CTA whose share holds tile x.
 static __device__ __noinline__ uint32_t paged_cta_of(uint64_t total, uint32_t ctas, uint64_t x) {
-    uint64_t c = x * ctas / total;
-    while (total * (c + 1) / ctas <= x) c++;
-    while (total * c / ctas > x) c--;
-    return uint32_t(c);
+    uint32_t c = total < (1u << 24) ? uint32_t(x) * ctas / uint32_t(total) : uint32_t(x * ctas / total);
+    while (paged_cut(total, c + 1, ctas) <= x) c++;
+    while (paged_cut(total, c, ctas) > x) c--;
+    return c;
 }
 // The CTAs that an item's tiles lie in: the first, and how many.
 __device__ __forceinline__ uint2 paged_ctas_of(const PagedShare &s, const PagedItem &it) {
@@ -142,56 +148,64 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
     const PagedTiles<T> tiles{tpt};
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
     uint64_t total = 0, x0 = 0;
+    // The sum of all sequences' tiles first, then which one holds x0; with no more sequences than threads the sums at hand serve both.
+    const bool once = a.seqs <= threads;
 #pragma unroll 1
-    for (int pass = 0; pass < 2; pass++) { // the sum first, then who holds x0
+    for (int pass = once ? 1 : 0; pass < 2; pass++) {
         uint64_t carry = 0;
+#pragma unroll 1
         for (uint32_t base = 0; base < a.seqs; base += threads) {
             const uint32_t s = base + tid;
             uint64_t cost = 0;
+            PagedSeq q;
+            q.row0 = q.n = q.kv = 0;
             if (s < a.seqs) {
-                const PagedSeq q = paged_seq(a, s);
+                q = paged_seq(a, s);
                 if (q.n) cost = a.kv_heads * tiles.per_head(q);
             }
             uint64_t v = cost;
+            if (a.seqs > 1) {
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint64_t y = __shfl_up_sync(0xffffffffu, v, d);
-                if (lane >= uint32_t(d)) v += y;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint64_t y = __shfl_up_sync(0xffffffffu, v, d);
+                    if (lane >= uint32_t(d)) v += y;
+                }
             }
-            if (lane == 31) scratch[warp] = v;
+            if (a.seqs == 1 ? tid == 0 : lane == 31) scratch[warp] = v;
             __syncthreads();
             uint64_t before = carry, all = 0;
+            if (a.seqs == 1) {
+                all = scratch[0];
+            } else {
 #pragma unroll 1
-            for (uint32_t w = 0; w < warps; w++) {
-                if (w < warp) before += scratch[w];
-                all += scratch[w];
+                for (uint32_t w = 0; w < warps; w++) {
+                    if (w < warp) before += scratch[w];
+                    all += scratch[w];
+                }
             }
             v += before; // inclusive
-            if (pass == 1 && cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost;
-            if (pass == 0 && a.seqs <= threads) { // one chunk: the sums at hand serve both passes
-                total = carry + all;
-                const uint64_t ctas = min(uint64_t(gridDim.x), max(uint64_t(1), (total + min_tiles - 1) / min_tiles));
-                x0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
-                if (cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost;
+            if (once || pass == 0) total = carry + all;
+            if (once) {
+                const uint32_t ctas = paged_ctas(total, min_tiles);
+                x0 = blockIdx.x < ctas ? paged_cut(total, blockIdx.x, ctas) : total;
             }
+            if (pass == 1 && cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost, share->q = q;
             carry += all;
             __syncthreads();
         }
-        total = carry;
-        const uint64_t ctas = min(uint64_t(gridDim.x), max(uint64_t(1), (total + min_tiles - 1) / min_tiles));
-        x0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+        const uint32_t ctas = paged_ctas(total, min_tiles);
+        x0 = blockIdx.x < ctas ? paged_cut(total, blockIdx.x, ctas) : total;
         if (tid == 0) {
-            share->total = total, share->ctas = uint32_t(ctas), share->x0 = x0;
-            share->x1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+            share->total = total, share->ctas = ctas, share->x0 = x0;
+            share->x1 = blockIdx.x < ctas ? paged_cut(total, blockIdx.x + 1, ctas) : total;
         }
-        if (a.seqs <= threads) break;
     }
     __syncthreads();
     if (warp == 0 && x0 < total) {
-        const PagedSeq q = paged_seq(a, share->seq);
-        const uint64_t per = tiles.per_head(q);
-        const uint32_t head = uint32_t((x0 - share->head_base) / per);
-        const uint64_t rest = x0 - share->head_base - uint64_t(head) * per;
+        const PagedSeq q = share->q;
+        const uint64_t per = tiles.per_head(q), rest_all = x0 - share->head_base;
+        const uint32_t head = rest_all >> 32 || per >> 32 ? uint32_t(rest_all / per) : uint32_t(rest_all) / uint32_t(per);
+        const uint64_t rest = rest_all - uint64_t(head) * per;
         uint32_t lo = 0, hi = tiles.row_tiles(q); // the last r with before(r) <= rest, 32 candidates at a time
         while (hi - lo > 1) {
             const uint32_t step = (hi - lo + 31) / 32, r = lo + lane * step;
@@ -199,7 +213,8 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
             lo += (__popc(le) - 1) * step;
             hi = min(hi, lo + step);
         }
-        if (lane == 0) share->head = head, share->rtile = lo;
+        const uint32_t kt0 = uint32_t(rest - tiles.before(q, lo));
+        if (lane == 0) share->head = head, share->rtile = lo, share->kt0 = kt0;
     }
     __syncthreads();
 }

@@ -300,7 +300,7 @@ class Case:
         want, b = self.ref()
         total = self.starts[-1]
         assert np.isfinite(got[:total]).all()
-        many = self.max_rows * (self.heads // self.kv_heads) > 32
+        many = self.max_rows * (self.heads // self.kv_heads) > 16
         lim = bound(self.out_dt, self.q_dt, want, b, max(self.kv_lens), self.dim, many)
         off = np.abs(got - want)[:total] / lim[:total]
         assert off.size == 0 or off.max() <= 1.0, (off.max(), np.unravel_index(off.argmax(), off.shape))
