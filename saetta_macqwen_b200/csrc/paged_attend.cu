@@ -41,7 +41,7 @@ struct PdLayout {
     static constexpr int kRow = 128 + 4;                      // floats of one row of the exchange buffer
     static constexpr int kExchange = 8 * 8 * kRow * 4;        // 8 warps x 8 rows of 128 dims
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * kPages * 8 /*scales*/ + 3072 /*barriers, statistics*/;
+    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * kPages * 8 /*scales*/ + 3072 /*barriers, items, statistics*/;
 };
 static_assert(PdLayout<256, 2>::kSmem <= 227 * 1024 && PdLayout<128, 2>::kSmem <= 227 * 1024, "fits a CTA's shared memory");
 
@@ -65,6 +65,27 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     return v;
 }
 
+// All consumers: whether `yes` holds for each of them.
+__device__ __forceinline__ bool consumers_all(bool yes) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r)
+                 : "r"(uint32_t(yes))
+                 : "memory");
+    return r;
+}
+
+// What the consumers need of an item; the producer walks the items and leaves this in a ring of shared memory.
+struct PdItem {
+    uint32_t kt0, kt1;    // key tiles; kt0 == kt1: no more items
+    int32_t lim0, vis;    // keys that the first and the last token see
+    uint32_t row0, ntok;  // first row of q, tokens
+    uint32_t head;
+    uint32_t c0, parts;   // the CTAs that the item lies in
+    uint32_t pad;
+};
+constexpr int kPdItems = 4;
+
 template <int D, int NT>
 __global__ void __launch_bounds__(kPdThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedArgs a, const uint32_t tpt) {
@@ -75,9 +96,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     float *xch = reinterpret_cast<float *>(ring + L::kRing);                  // [8 warps][8 rows][kRow]
     float2 *scl = reinterpret_cast<float2 *>(ring + L::kRing + L::kExchange); // [stage][page]
     uint64_t *full = reinterpret_cast<uint64_t *>(scl + L::kStages * L::kPages), *empty = full + L::kStages;
-    uint64_t *scratch = empty + L::kStages; // 40 words
+    uint64_t *item_full = empty + L::kStages, *item_empty = item_full + kPdItems;
+    uint64_t *scratch = item_empty + kPdItems; // 40 words
     PagedShare *share = reinterpret_cast<PagedShare *>(scratch + 40);
-    float *wm = reinterpret_cast<float *>(share + 1); // [8][R] maxima, then sums, then weights; [R] joint maximum and sum
+    PdItem *items = reinterpret_cast<PdItem *>(share + 1);
+    float *wm = reinterpret_cast<float *>(items + kPdItems); // [8][R] maxima, then sums, then weights; [R] joint maximum and sum
     float *wl = wm + 8 * 16, *ww = wl + 8 * 16, *rm = ww + 8 * 16, *rl = rm + 16, *wv = rl + 16;
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(wv + 8);
     volatile uint32_t *never_set = abort_flag + 1;
@@ -86,6 +109,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < L::kStages; s++) mbar_init(&full[s], 33), mbar_init(&empty[s], 4);
+        for (int s = 0; s < kPdItems; s++) mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], 8);
         *abort_flag = 0, *never_set = 0;
         mbar_fence_init();
     }
@@ -99,34 +123,44 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     };
     const uint32_t bt = min(a.block_tokens, uint32_t(kTile)); // keys of one copy
     const uint32_t G = a.group;
-    PagedWalk<kTile> walk(a, *share, tpt);
-    PagedItem it;
 
     // registers: 256 x 232 + 128 x 40 = the 384 x 168 of the launch
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp > 8) return;
         // ------------------------------------------------------------ producer
-        uint32_t g = 0;
+        PagedWalk<kTile> walk(a, *share, tpt);
+        PagedItem it;
+        uint32_t g = 0, ni = 0;
         bool ok = true;
+        const uint32_t per_tile = kTile / bt;
         while (ok && walk.next(it)) {
             const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
             const uint32_t keys = walk.tiles.keys(it.q, it.rtile);
-            const uint32_t per_tile = kTile / bt;
             auto block_of = [&](uint32_t kt) -> int32_t { // of this lane's page of a tile; -2: none
                 const uint32_t key = kt * kTile + lane * bt;
-                return lane < per_tile && key < keys ? table[key / a.block_tokens] : -2;
+                return lane < per_tile && kt < it.kt1 && key < keys ? table[key / a.block_tokens] : -2;
             };
-            int32_t next = block_of(it.kt0);
+            int32_t ahead[3] = {block_of(it.kt0), block_of(it.kt0 + 1), block_of(it.kt0 + 2)}; // a table entry is some 800 clocks away
+            if (!mbar_wait(&item_empty[ni % kPdItems], (ni / kPdItems & 1) ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); break; }
+            const uint2 span = it.kt0 == 0 && it.kt1 == it.tiles ? make_uint2(0, 1) : paged_ctas_of(*share, it);
+            if (lane == 0) {
+                items[ni % kPdItems] = PdItem{it.kt0, it.kt1, it.lim0, paged_visible(it), it.q.row0 + it.tok0, it.ntok, it.head, span.x, span.y, 0};
+                mbar_arrive(&item_full[ni % kPdItems]);
+            }
+            __syncwarp();
+            ni++;
+            for (uint32_t i = lane; i < it.ntok * G * (D / 64); i += 32) // the query rows on their way to L2 (128 bytes each, of a 16-bit row)
+                prefetch_l2(static_cast<const uint16_t *>(a.q) + (size_t(it.q.row0 + it.tok0 + i / (G * (D / 64))) * a.q_stride + size_t(it.head) * G * D + i % (G * (D / 64)) * 64) * (a.q_dtype == SAETTA_F32 ? 2 : 1));
             for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
                 const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
-                int32_t block = next;
-                if (kt + 1 < it.kt1) next = block_of(kt + 1);
-                if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); ok = false; break; }
+                const int32_t block = ahead[0];
+                ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = block_of(kt + 3);
                 const bool want = block != -2;
                 const bool good = want && uint32_t(block) < a.blocks;
                 if (want && !good) atomicOr(a.words, kStatusBadBlock);
                 const uint32_t pages = __popc(__ballot_sync(0xffffffffu, good));
+                if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); ok = false; break; }
                 if (lane == 0) mbar_expect_tx(&full[st], pages * 2 * bt * D);
                 __syncwarp();
                 if (good) {
@@ -138,9 +172,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 }
                 if (want) // a bad block's keys are marked by its scales
                     cp_async8(&scl[st * L::kPages + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
-                                                        : reinterpret_cast<const float *>(a.words + kPagedBadScale));
+                                                                : reinterpret_cast<const float *>(a.words + kPagedBadScale));
                 cp_async_arrive(&full[st]);
             }
+        }
+        if (ok && mbar_wait(&item_empty[ni % kPdItems], (ni / kPdItems & 1) ^ 1, abort_flag) && lane == 0) {
+            items[ni % kPdItems].kt0 = items[ni % kPdItems].kt1 = 0;
+            mbar_arrive(&item_full[ni % kPdItems]);
         }
         // let what was issued land before the shared memory goes
         const uint32_t from = g > L::kStages ? g - L::kStages : 0;
@@ -153,7 +191,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const uint32_t gi = lane >> 2, t = lane & 3, sub = warp & 3, team = warp >> 2;
     uint32_t g = 0;
     bool ok = true;
-    while (walk.next(it)) {
+    for (uint32_t ni = 0;; ni++) {
+        // (the consumers agree whether there is another item: they meet at barriers that have no bound)
+        if (!consumers_all(mbar_wait(&item_full[ni % kPdItems], ni / kPdItems & 1, abort_flag))) {
+            give_up(kStatusFullTimeout);
+            break;
+        }
+        const PdItem it = items[ni % kPdItems];
+        if (it.kt0 == it.kt1) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[ni % kPdItems]);
         // the item's query rows as B fragments, binary16 after a power of two that brings the row's largest to [128, 256)
         uint32_t qf[NT][D / 16][2];
         float rs[NT][2]; // of rows 2 t and 2 t + 1: that power undone, times the softmax scale in log2 units
@@ -168,7 +215,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             for (int c = 0; c < kSlabs * 4; c++) {
                 // chunk 2 t + j of a slab, its two halves
                 const uint32_t d = (c >> 2) * 128 + (2 * t + ((c >> 1) & 1)) * 16 + (c & 1) * 8;
-                if (live) paged_load_q8(a, size_t(it.q.row0 + it.tok0 + tok) * a.q_stride + size_t(hd) * D + d, x[c]);
+                if (live) paged_load_q8(a, size_t(it.row0 + tok) * a.q_stride + size_t(hd) * D + d, x[c]);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     if (!live) x[c][e] = 0.f;
@@ -206,7 +253,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[nt][i][e] = 0.f;
         }
-        const int32_t vis = paged_visible(it);
+        const int32_t vis = it.vis;
         for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
             if ((g & 1) != team) continue;
             const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
@@ -367,12 +414,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             ww[w * R + row] = ex2_approx(wm[w * R + row] - mu) * wv[w];
             if (w == 0) rm[row] = top, rl[row] = sum;
         }
-        const bool whole = it.kt0 == 0 && it.kt1 == it.tiles;
+        const bool whole = it.parts == 1;
         float *part = a.parts + (size_t(blockIdx.x) * 2 + (it.kt0 == 0 ? 1 : 0)) * a.part_floats;
         auto finish = [&](uint32_t row, uint32_t d, float4 v, float sum) { // one row's dims d .. d + 3, unnormalised
             const uint32_t tok = row / G, hd = it.head * G + row % G;
             if (tok >= it.ntok || row >= tpt * G) return;
-            const size_t at = size_t(it.q.row0 + it.tok0 + tok) * a.heads + hd;
+            const size_t at = size_t(it.row0 + tok) * a.heads + hd;
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum); // no key: 0; NaN stays
             v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
             if (a.q_and_gate) {
@@ -416,8 +463,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (tid < R) ml[tid * 2] = rm[tid], ml[tid * 2 + 1] = rl[tid];
             // The parts are joined by the last CTA to arrive, in the order of the CTAs; many of them in two rounds, groups of some first, because one CTA
             // reads no more than some 100 bytes a clock.
-            const uint2 span = paged_ctas_of(*share, it);
-            const uint32_t c0 = span.x, parts = span.y;
+            const uint32_t c0 = it.c0, parts = it.parts;
             uint32_t per = parts; // parts of a group
             if (parts > kPdGroup) {
                 per = 2;
@@ -432,13 +478,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 consumers_sync();
                 float top = -INFINITY, sum = 0.f;
                 if (tid < R) {
+#pragma unroll 4
                     for (uint32_t p = 0; p < n; p++) top = fmaxf(top, in[p * R + tid].x);
                     const float mu = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
                     for (uint32_t p = 0; p < n; p++) {
                         const float2 x = in[p * R + tid];
                         const float w = ex2_approx(x.x - mu);
                         in[p * R + tid].x = w;
-                        sum += x.y * w;
+                        sum = fmaf(x.y, w, sum);
                     }
                     rl[tid] = sum;
                 }

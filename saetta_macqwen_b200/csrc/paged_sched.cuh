@@ -57,7 +57,7 @@ struct PagedTiles {
         if (full != r) sum += count(q, r - 1);
         return sum;
     }
-    __device__ __forceinline__ uint64_t per_head(const PagedSeq &q) const { return before(q, row_tiles(q)); }
+    __device__ __forceinline__ uint64_t per_head(const PagedSeq &q) const { return q.n <= tpt ? count(q, 0) : before(q, row_tiles(q)); }
 };
 
 // One CTA's part of one item.
@@ -73,6 +73,7 @@ struct PagedItem {
 struct PagedShare {
     uint64_t total, x0, x1; // tiles of the launch, this CTA's
     uint64_t head_base;     // flat index of (seq, head 0, row tile 0)
+    uint64_t per_head;      // tiles of `seq` for each kv head
     uint32_t ctas;          // that have a share
     uint32_t seq, head, rtile, kt0; // where it begins
     PagedSeq q;             // of `seq`
@@ -156,12 +157,12 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
 #pragma unroll 1
         for (uint32_t base = 0; base < a.seqs; base += threads) {
             const uint32_t s = base + tid;
-            uint64_t cost = 0;
+            uint64_t cost = 0, per = 0;
             PagedSeq q;
             q.row0 = q.n = q.kv = 0;
             if (s < a.seqs) {
                 q = paged_seq(a, s);
-                if (q.n) cost = a.kv_heads * tiles.per_head(q);
+                if (q.n) cost = a.kv_heads * (per = tiles.per_head(q));
             }
             uint64_t v = cost;
             if (a.seqs > 1) {
@@ -189,7 +190,7 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
                 const uint32_t ctas = paged_ctas(total, min_tiles);
                 x0 = blockIdx.x < ctas ? paged_cut(total, blockIdx.x, ctas) : total;
             }
-            if (pass == 1 && cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost, share->q = q;
+            if (pass == 1 && cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost, share->q = q, share->per_head = per;
             carry += all;
             __syncthreads();
         }
@@ -203,7 +204,7 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
     __syncthreads();
     if (warp == 0 && x0 < total) {
         const PagedSeq q = share->q;
-        const uint64_t per = tiles.per_head(q), rest_all = x0 - share->head_base;
+        const uint64_t per = share->per_head, rest_all = x0 - share->head_base;
         const uint32_t head = rest_all >> 32 || per >> 32 ? uint32_t(rest_all / per) : uint32_t(rest_all) / uint32_t(per);
         const uint64_t rest = rest_all - uint64_t(head) * per;
         uint32_t lo = 0, hi = tiles.row_tiles(q); // the last r with before(r) <= rest, 32 candidates at a time
@@ -213,7 +214,7 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
             lo += (__popc(le) - 1) * step;
             hi = min(hi, lo + step);
         }
-        const uint32_t kt0 = uint32_t(rest - tiles.before(q, lo));
+        const uint32_t kt0 = uint32_t(rest - (lo ? tiles.before(q, lo) : 0));
         if (lane == 0) share->head = head, share->rtile = lo, share->kt0 = kt0;
     }
     __syncthreads();
