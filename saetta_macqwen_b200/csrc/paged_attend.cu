@@ -6,7 +6,7 @@
 // tensor cores as they are (an e4m3 value is a binary16 value).  Bound by the cache's bytes, 2 * head_dim for each key and
 // kv head; the rest is arranged so that these stream without a pause:
 //
-//  * One CTA for each SM takes an equal share of all key tiles (paged_sched.cuh); a producer warp keeps a ring of
+//  * One CTA for each SM takes an equal share of all key tiles (paged_sched.cuh); producer warps keep a ring of
 //    tiles of K and V in flight (64 keys with head dim 256, 128 with 128; TMA tensor copies of whole pages, 128-byte
 //    swizzle: 160 KB on the way) and the pages' scales beside them (8-byte asynchronous copies).
 //  * Eight consumer warps, four for each tile, 16 or 32 keys a warp, each with its own running maximum, sum and accumulators: no
@@ -38,6 +38,7 @@ struct PdLayout {
     static constexpr int kStage = 2 * kSide;       // 32 KB
     static constexpr int kStages = 5;
     static constexpr int kPages = kTile / 16;      // of a tile, at most
+    static_assert(kRows * D / 4 >= 256, "every consumer has values to join");
     static constexpr int kRow = 128 + 4;                      // floats of one row of the exchange buffer
     static constexpr int kExchange = 8 * 8 * kRow * 4;        // 8 warps x 8 rows of 128 dims
     static constexpr int kRing = kStages * kStage;
@@ -50,7 +51,6 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(w)));
     return h;
 }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void cp_async8(void *dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
@@ -108,7 +108,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int s = 0; s < L::kStages; s++) mbar_init(&full[s], 33), mbar_init(&empty[s], 4);
+        for (int s = 0; s < L::kStages; s++) mbar_init(&full[s], 34), mbar_init(&empty[s], 4);
         for (int s = 0; s < kPdItems; s++) mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], 8);
         *abort_flag = 0, *never_set = 0;
         mbar_fence_init();
@@ -127,56 +127,57 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     // registers: 256 x 232 + 128 x 40 = the 384 x 168 of the launch
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp > 8) return;
-        // ------------------------------------------------------------ producer
+        if (warp == 11) return;
+        // ------------------------------------------------------------ producers: warp 8 the items and the keys, 9 the values, 10 the scales
+        // (One warp for all three took 2200 clocks for a tile of 8 pages, which the memory delivers in 1400.)
         PagedWalk<kTile> walk(a, *share, tpt);
         PagedItem it;
         uint32_t g = 0, ni = 0;
         bool ok = true;
         const uint32_t per_tile = kTile / bt;
+        PagedPages pages;
         while (ok && walk.next(it)) {
-            const int32_t *table = a.tables + size_t(it.seq) * a.table_stride;
             const uint32_t keys = walk.tiles.keys(it.q, it.rtile);
-            auto block_of = [&](uint32_t kt) -> int32_t { // of this lane's page of a tile; -2: none
-                const uint32_t key = kt * kTile + lane * bt;
-                return lane < per_tile && kt < it.kt1 && key < keys ? table[key / a.block_tokens] : -2;
-            };
-            int32_t ahead[3] = {block_of(it.kt0), block_of(it.kt0 + 1), block_of(it.kt0 + 2)}; // a table entry is some 800 clocks away
-            if (!mbar_wait(&item_empty[ni % kPdItems], (ni / kPdItems & 1) ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); break; }
-            const uint2 span = it.kt0 == 0 && it.kt1 == it.tiles ? make_uint2(0, 1) : paged_ctas_of(*share, it);
-            if (lane == 0) {
-                items[ni % kPdItems] = PdItem{it.kt0, it.kt1, it.lim0, paged_visible(it), it.q.row0 + it.tok0, it.ntok, it.head, span.x, span.y, 0};
+            pages.begin(a, it.seq, keys, bt, it.kt0 * per_tile);
+            if (warp == 8 && !mbar_wait(&item_empty[ni % kPdItems], (ni / kPdItems & 1) ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); break; }
+            PdItem *item = &items[ni % kPdItems];
+            if (warp == 8 && lane == 0) {
+                *item = PdItem{it.kt0, it.kt1, it.lim0, paged_visible(it), it.q.row0 + it.tok0, it.ntok, it.head, 0, 1, 0};
                 mbar_arrive(&item_full[ni % kPdItems]);
             }
             __syncwarp();
             ni++;
-            for (uint32_t i = lane; i < it.ntok * G * (D / 64); i += 32) // the query rows on their way to L2 (128 bytes each, of a 16-bit row)
-                prefetch_l2(static_cast<const uint16_t *>(a.q) + (size_t(it.q.row0 + it.tok0 + i / (G * (D / 64))) * a.q_stride + size_t(it.head) * G * D + i % (G * (D / 64)) * 64) * (a.q_dtype == SAETTA_F32 ? 2 : 1));
+            for (uint32_t tk = 0; warp == 9 && tk < it.ntok; tk++) { // the query rows on their way to L2
+                const uint32_t el = a.q_dtype == SAETTA_F32 ? 4 : 2;
+                const char *row = static_cast<const char *>(a.q) + (size_t(it.q.row0 + it.tok0 + tk) * a.q_stride + size_t(it.head) * G * D) * el;
+                for (uint32_t at = lane * 128; at < G * D * el; at += 32 * 128) prefetch_l2(row + at);
+            }
             for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
-                const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
-                const int32_t block = ahead[0];
-                ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = block_of(kt + 3);
-                const bool want = block != -2;
-                const bool good = want && uint32_t(block) < a.blocks;
-                if (want && !good) atomicOr(a.words, kStatusBadBlock);
-                const uint32_t pages = __popc(__ballot_sync(0xffffffffu, good));
-                if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); ok = false; break; }
-                if (lane == 0) mbar_expect_tx(&full[st], pages * 2 * bt * D);
-                __syncwarp();
-                if (good) {
-                    uint8_t *dst = ring + st * L::kStage + lane * bt * D;
-                    const uint32_t key = kt * kTile + lane * bt;
-                    const int row = int((uint32_t(block) * a.kv_heads + it.head) * a.block_tokens + (key & (a.block_tokens - 1)));
-                    tma_load_3d(dst, &map_k, &full[st], 0, row, 0);
-                    tma_load_3d(dst + L::kSide, &map_v, &full[st], 0, row, 0);
+                const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1, key0 = kt * kTile;
+                const int32_t block = pages.of(kt * per_tile); // of this lane's copy
+                const bool want = lane < per_tile && key0 + lane * bt < keys, good = want && uint32_t(block) < a.blocks;
+                if (warp == 8 && kt + 1 == it.kt1 && it.kt1 - it.kt0 < it.tiles) { // where the parts are (read after the last tile)
+                    const uint2 span = paged_ctas_of(*share, it);
+                    if (lane == 0) item->c0 = span.x, item->parts = span.y;
                 }
-                if (want) // a bad block's keys are marked by its scales
-                    cp_async8(&scl[st * L::kPages + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
-                                                                : reinterpret_cast<const float *>(a.words + kPagedBadScale));
-                cp_async_arrive(&full[st]);
+                if (!mbar_wait(&empty[st], ph ^ 1, abort_flag)) { give_up(kStatusEmptyTimeout); ok = false; break; }
+                if (warp == 10) {
+                    if (want && !good) atomicOr(a.words, kStatusBadBlock);
+                    if (want) // a bad block's keys are marked by its scales
+                        cp_async8(&scl[st * L::kPages + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
+                                                                    : reinterpret_cast<const float *>(a.words + kPagedBadScale));
+                    cp_async_arrive(&full[st]);
+                    continue;
+                }
+                const uint32_t copies = __popc(__ballot_sync(0xffffffffu, good));
+                if (lane == 0) mbar_expect_tx(&full[st], copies * bt * D);
+                __syncwarp();
+                if (good)
+                    tma_load_3d(ring + st * L::kStage + (warp == 9 ? L::kSide : 0) + lane * bt * D, warp == 9 ? &map_v : &map_k, &full[st], 0,
+                                int((uint32_t(block) * a.kv_heads + it.head) * a.block_tokens + ((key0 + lane * bt) & (a.block_tokens - 1))), 0);
             }
         }
-        if (ok && mbar_wait(&item_empty[ni % kPdItems], (ni / kPdItems & 1) ^ 1, abort_flag) && lane == 0) {
+        if (warp == 8 && ok && mbar_wait(&item_empty[ni % kPdItems], (ni / kPdItems & 1) ^ 1, abort_flag) && lane == 0) {
             items[ni % kPdItems].kt0 = items[ni % kPdItems].kt1 = 0;
             mbar_arrive(&item_full[ni % kPdItems]);
         }
@@ -199,8 +200,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         const PdItem it = items[ni % kPdItems];
         if (it.kt0 == it.kt1) break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&item_empty[ni % kPdItems]);
         // the item's query rows as B fragments, binary16 after a power of two that brings the row's largest to [128, 256)
         uint32_t qf[NT][D / 16][2];
         float rs[NT][2]; // of rows 2 t and 2 t + 1: that power undone, times the softmax scale in log2 units
@@ -414,7 +413,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             ww[w * R + row] = ex2_approx(wm[w * R + row] - mu) * wv[w];
             if (w == 0) rm[row] = top, rl[row] = sum;
         }
-        const bool whole = it.parts == 1;
+        const uint32_t c0 = items[ni % kPdItems].c0, parts = items[ni % kPdItems].parts;
+        const bool whole = parts == 1;
         float *part = a.parts + (size_t(blockIdx.x) * 2 + (it.kt0 == 0 ? 1 : 0)) * a.part_floats;
         auto finish = [&](uint32_t row, uint32_t d, float4 v, float sum) { // one row's dims d .. d + 3, unnormalised
             const uint32_t tok = row / G, hd = it.head * G + row % G;
@@ -463,7 +463,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (tid < R) ml[tid * 2] = rm[tid], ml[tid * 2 + 1] = rl[tid];
             // The parts are joined by the last CTA to arrive, in the order of the CTAs; many of them in two rounds, groups of some first, because one CTA
             // reads no more than some 100 bytes a clock.
-            const uint32_t c0 = it.c0, parts = it.parts;
             uint32_t per = parts; // parts of a group
             if (parts > kPdGroup) {
                 per = 2;
@@ -471,64 +470,66 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             const uint32_t groups = (parts + per - 1) / per, mine = (blockIdx.x - c0) / per;
             auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
-            // joins parts lo, lo + step, ... (n of them): into part lo, or the output
-            auto join = [&](uint32_t lo, uint32_t step, uint32_t n, bool last) {
-                float2 *in = reinterpret_cast<float2 *>(xch); // [n][R] maxima and sums; the maxima become weights
-                for (uint32_t i = tid; i < n * R; i += 256) in[i] = __ldcg(reinterpret_cast<const float2 *>(part_of(lo + i / R * step) + R * D) + i % R);
-                consumers_sync();
-                float top = -INFINITY, sum = 0.f;
-                if (tid < R) {
-#pragma unroll 4
-                    for (uint32_t p = 0; p < n; p++) top = fmaxf(top, in[p * R + tid].x);
-                    const float mu = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-                    for (uint32_t p = 0; p < n; p++) {
-                        const float2 x = in[p * R + tid];
-                        const float w = ex2_approx(x.x - mu);
-                        in[p * R + tid].x = w;
-                        sum = fmaf(x.y, w, sum);
-                    }
-                    rl[tid] = sum;
-                }
-                consumers_sync();
+            // parts lo, lo + step, ... (n of them) are joined: into part lo, or the output
+            uint32_t lo = mine * per, step = 1, n = min(per, parts - lo);
+            // a group's counter: by its first CTA, which may begin another item's tail as well
+            uint32_t *counter = a.words + kPagedCounters + (mine ? gridDim.x : 0) + c0 + lo;
 #pragma unroll 1
-                for (uint32_t i = tid; i < R * D / 4; i += 256) {
-                    const uint32_t row = i * 4 / D, d = i * 4 % D;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (uint32_t p = 0; p < n; p++) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(lo + p * step) + row * D + d));
-                        const float wt = in[p * R + row].x;
-                        v.x = fmaf(x.x, wt, v.x), v.y = fmaf(x.y, wt, v.y), v.z = fmaf(x.z, wt, v.z), v.w = fmaf(x.w, wt, v.w);
-                    }
-                    if (last) finish(row, d, v, rl[row]);
-                    else *reinterpret_cast<float4 *>(part_of(lo) + row * D + d) = v;
-                }
-                if (!last && tid < R) *reinterpret_cast<float2 *>(part_of(lo) + R * D + tid * 2) = make_float2(top, sum);
-            };
-            // whether this CTA is the last of `n` to come to the counter, which it then sets back
-            auto last_of = [&](uint32_t *counter, uint32_t n) {
-                __threadfence();
+            for (bool last = groups == 1;; last = true) {
                 consumers_sync();
                 if (tid == 0) {
+                    __threadfence(); // (the others' writes too: they came before the barrier)
                     const uint32_t k = atomicAdd(counter, 1) + 1;
                     if (k == n) *counter = 0;
+                    __threadfence();
                     *arrived = k;
                 }
                 consumers_sync();
-                const bool yes = *arrived == n;
-                if (yes) __threadfence();
-                consumers_sync();
-                return yes;
-            };
-            uint32_t *counters = a.words + kPagedCounters;
-            // a group's counter: by its first CTA, which may begin another item's tail as well
-            if (last_of(counters + (mine ? gridDim.x : 0) + c0 + mine * per, min(per, parts - mine * per))) {
-                join(mine * per, 1, min(per, parts - mine * per), groups == 1);
-                if (groups > 1 && last_of(counters + 2 * gridDim.x + c0, groups)) join(0, per, groups, true);
+                if (*arrived != n) break;
+                float4 x[kPdGroup + 1];
+                float2 *in = reinterpret_cast<float2 *>(xch); // [n][R] maxima and sums; the maxima become weights
+                for (uint32_t i = tid; i < n * R; i += 256) in[i] = __ldcg(reinterpret_cast<const float2 *>(part_of(lo + i / R * step) + R * D) + i % R);
+                float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+                for (uint32_t i = tid; i < R * D / 4; i += 256) {
+                    const uint32_t row = i * 4 / D, d = i * 4 % D;
+#pragma unroll
+                    for (uint32_t p = 0; p <= kPdGroup; p++)
+                        if (p < n) x[p] = __ldcg(reinterpret_cast<const float4 *>(part_of(lo + p * step)) + i);
+                    if (i == tid) { // the weights, while the first values are on their way
+                        consumers_sync();
+                        if (tid < R) {
+#pragma unroll 4
+                            for (uint32_t p = 0; p < n; p++) top = fmaxf(top, in[p * R + tid].x);
+                            const float mu = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+                            for (uint32_t p = 0; p < n; p++) {
+                                const float2 y = in[p * R + tid];
+                                const float w = ex2_approx(y.x - mu);
+                                in[p * R + tid].x = w;
+                                sum = fmaf(y.y, w, sum);
+                            }
+                            rl[tid] = sum;
+                        }
+                        consumers_sync();
+                    }
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (uint32_t p = 0; p <= kPdGroup; p++)
+                        if (p < n) {
+                            const float wt = in[p * R + row].x;
+                            v.x = fmaf(x[p].x, wt, v.x), v.y = fmaf(x[p].y, wt, v.y), v.z = fmaf(x[p].z, wt, v.z), v.w = fmaf(x[p].w, wt, v.w);
+                        }
+                    if (last) finish(row, d, v, rl[row]);
+                    else reinterpret_cast<float4 *>(part_of(lo))[i] = v;
+                }
+                if (last) break;
+                if (tid < R) *reinterpret_cast<float2 *>(part_of(lo) + R * D + tid * 2) = make_float2(top, sum);
+                lo = 0, step = per, n = groups, counter = a.words + kPagedCounters + 2 * gridDim.x + c0;
             }
         }
         consumers_sync(); // statistics and exchange buffer are free for the next item
+        if (lane == 0) mbar_arrive(&item_empty[ni % kPdItems]);
     }
 }
 

@@ -73,11 +73,6 @@ struct PpLayout {
 // Descriptors come as their low words; the high word, the same for all (stride 1024 bytes, 128-byte swizzle), is an immediate.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ bool elect_one() {
-    uint32_t yes;
-    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(yes));
-    return yes;
-}
 __device__ __forceinline__ void tc_mma8(uint32_t d_tmem, uint32_t adesc, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
@@ -283,24 +278,30 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             // (A K stage is free once the scores that use it are done, and those wait for no value product later than the one two
             // tiles before them.)
             const uint32_t bt = min(a.block_tokens, uint32_t(kPpKeys)), per_tile = kPpKeys / bt;
-            const uint32_t page = lane / kSlabs, slab = lane % kSlabs;
             PagedWalk<kPpKeys> walk(a, *share, tpt);
             const uint32_t tiles = walk.end;
-            uint32_t ni = 0, kk = 0, kk1 = 0;
-            int row[kPpAhead + 2] = {-1, -1, -1, -1}; // this lane's row of the cache for the next tile, the tile at hand, and those before; -1: none
-            const int32_t *table = nullptr;
-            uint32_t keys = 0, head = 0;
-            for (uint32_t i = 0; i < tiles + kPpAhead + 1; i++) { // the copies of a tile are issued a step after its page has been looked up
+            uint32_t ni = 0, kk = 0, kk1 = 0, keys = 0, head = 0;
+            int row[kPpAhead + 1] = {-1, -1, -1}; // of this lane's copy in the cache, of the tile at hand and those before; -1: none
+            PagedPages pages;
+            auto copy = [&](const CUtensorMap *map, uint64_t *full, uint8_t *dst, int mine) { // a lane for each page and slab
+                const int r = __shfl_sync(0xffffffffu, mine, lane / kSlabs);
+                const bool good = lane / kSlabs < per_tile && r >= 0;
+                const uint32_t copies = __popc(__ballot_sync(0xffffffffu, good));
+                if (lane == 0) mbar_expect_tx(full, copies * bt * 128);
+                __syncwarp();
+                if (good) tma_load_3d(dst + lane % kSlabs * (kPpKeys * 128) + lane / kSlabs * bt * 128, map, full, 0, r, int(lane % kSlabs));
+            };
+            for (uint32_t i = 0; i < tiles + kPpAhead; i++) {
 #pragma unroll
-                for (int k = kPpAhead + 1; k > 0; k--) row[k] = row[k - 1];
+                for (int k = kPpAhead; k > 0; k--) row[k] = row[k - 1];
                 if (i < tiles) {
                     if (kk == kk1) {
                         PagedItem it;
                         walk.next(it);
-                        PP_WAIT(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1);
-                        const uint2 span = paged_ctas_of(*share, it);
                         kk = it.kt0, kk1 = it.kt1, keys = walk.tiles.keys(it.q, it.rtile), head = it.head;
-                        table = a.tables + size_t(it.seq) * a.table_stride;
+                        pages.begin(a, it.seq, keys, bt, kk * per_tile);
+                        PP_WAIT(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1);
+                        const uint2 span = it.kt0 == 0 && it.kt1 == it.tiles ? make_uint2(0, 1) : paged_ctas_of(*share, it);
                         if (lane == 0) {
                             items[ni % kPpItems] = PpItem{it.kt0, it.kt1, it.lim0, it.seq, it.head, it.q.row0 + it.tok0, it.ntok, keys, span.x | span.y << 16, 0.f};
                             mbar_arrive(&item_full[ni % kPpItems]);
@@ -308,30 +309,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         __syncwarp();
                         ni++;
                     }
-                    const uint32_t key = kk * kPpKeys + page * bt;
-                    row[0] = -1;
-                    if (page < per_tile && key < keys) {
-                        const uint32_t block = uint32_t(table[key / a.block_tokens]);
-                        if (block < a.blocks) row[0] = int((block * a.kv_heads + head) * a.block_tokens);
-                    }
+                    const uint32_t block = uint32_t(pages.of(kk * per_tile));
+                    row[0] = lane < per_tile && kk * kPpKeys + lane * bt < keys && block < a.blocks ? int((block * a.kv_heads + head) * a.block_tokens) : -1;
                     kk++;
+                    const uint32_t st = i % NK;
+                    PP_WAIT(&k_empty[st], (i / NK & 1) ^ 1);
+                    copied_k = i + 1;
+                    copy(&map_k, &k_full[st], ring + st * L::kStage, row[0]);
                 }
-                const uint32_t dst = slab * (kPpKeys * 128) + page * bt * 128;
-                if (i >= 1 && i <= tiles) {
-                    const uint32_t g = i - 1, st = g % NK, n = __popc(__ballot_sync(0xffffffffu, row[1] >= 0));
-                    PP_WAIT(&k_empty[st], (g / NK & 1) ^ 1);
-                    if (lane == 0) mbar_expect_tx(&k_full[st], n * bt * 128);
-                    copied_k = g + 1;
-                    __syncwarp();
-                    if (row[1] >= 0) tma_load_3d(ring + st * L::kStage + dst, &map_k, &k_full[st], 0, row[1], int(slab));
-                }
-                if (i >= kPpAhead + 1) {
-                    const uint32_t g = i - kPpAhead - 1, st = g % NV, n = __popc(__ballot_sync(0xffffffffu, row[kPpAhead + 1] >= 0));
+                if (i >= kPpAhead) {
+                    const uint32_t g = i - kPpAhead, st = g % NV;
                     PP_WAIT(&v_empty[st], (g / NV & 1) ^ 1);
-                    if (lane == 0) mbar_expect_tx(&v_full[st], n * bt * 128);
                     copied_v = g + 1;
-                    __syncwarp();
-                    if (row[kPpAhead + 1] >= 0) tma_load_3d(ring_v + st * L::kStage + dst, &map_v, &v_full[st], 0, row[kPpAhead + 1], int(slab));
+                    copy(&map_v, &v_full[st], ring_v + st * L::kStage, row[kPpAhead]);
                 }
             }
             PP_WAIT(&item_empty[ni % kPpItems], (ni / kPpItems & 1) ^ 1);

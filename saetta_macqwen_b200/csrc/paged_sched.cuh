@@ -220,6 +220,35 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
     __syncthreads();
 }
 
+// The pages of an item's tiles, for the warp that copies them: 32 table entries at a time in a register of each lane, and the 32 after them on
+// their way (an entry is some 800 clocks away, and the copies of a tile take 200).
+struct PagedPages {
+    const int32_t *table;
+    uint32_t entries, base, shift; // entries of the table in use; first one in `now`; log2 of the copies to an entry
+    int32_t now, next;             // -1: none
+    __device__ __forceinline__ int32_t load(uint32_t first) const {
+        const uint32_t i = first + (threadIdx.x & 31);
+        return i < entries ? table[i] : -1;
+    }
+    // `copy`: number of the first copy (of bt keys) that will be asked for
+    __device__ __forceinline__ void begin(const PagedArgs &a, uint32_t seq, uint32_t keys, uint32_t bt, uint32_t copy) {
+        table = a.tables + size_t(seq) * a.table_stride;
+        entries = (keys + a.block_tokens - 1) / a.block_tokens;
+        shift = a.block_tokens > bt ? __ffs(int(a.block_tokens / bt)) - 1 : 0;
+        base = (copy >> shift) & ~31u;
+        now = load(base), next = load(base + 32);
+    }
+    // The block of copy number `copy` + lane: asked for in rising order; a tile's copies lie within one such group of 32.
+    __device__ __forceinline__ int32_t of(uint32_t copy) {
+        const uint32_t first = copy >> shift;
+        if (first >= base + 32) {
+            base += 32;
+            now = next, next = load(base + 32);
+        }
+        return __shfl_sync(0xffffffffu, now, ((copy + (threadIdx.x & 31)) >> shift) - base);
+    }
+};
+
 // Four values of an output row.
 __device__ __forceinline__ void paged_store4(const PagedArgs &a, size_t i, float x, float y, float z, float w) {
     if (a.out_dtype == SAETTA_F32) {
