@@ -222,69 +222,79 @@ __device__ __forceinline__ float pow2_scale(float amax) {
     return __uint_as_float(uint32_t(max(e, 1)) << 23);
 }
 
-// A warp for each (run of rows in one block, kv head, side).  Row r leads a run where the row before it lies in another
-// block; the other rows' warps end at once.  Bound by memory: rows in, codes out, each once (the second pass over a run,
-// which needs its largest value, hits the caches).
+// A CTA for each (16 rows of the call, kv head, side): it takes the runs (rows of one block, one behind the other) that begin there, long ones with all
+// of its warps, short ones with a warp each; a row leads a run where the row before it lies in another block.  Bound by memory: rows
+// in, codes out, each once (the second pass over a run, which needs its largest value, hits the caches).  A warp for each run
+// took 45 us for 17413 bfloat16 rows of 2 x 256 in blocks of 64: too few loads on their way.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
-    constexpr int kLanes = D / 8;     // lanes of one row
-    constexpr int kRows = 32 / kLanes; // rows a warp takes at once
-    pdl_wait();
-    const uint32_t unit = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-    const uint32_t per_row = a.kv_heads * 2;
-    const uint32_t row = unit / per_row, rest = unit % per_row, head = rest >> 1, side = rest & 1;
-    if (row >= a.rows) return;
+    constexpr uint32_t kLanes = D / 8;      // lanes of one row
+    constexpr uint32_t kRows = 32 / kLanes; // rows a warp takes at once
+    __shared__ float red[8];
+    const uint32_t per_row = a.kv_heads * 2, rest = blockIdx.x % per_row, head = rest >> 1, side = rest & 1;
+    const uint32_t row0 = blockIdx.x / per_row * 16, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t B = 1u << a.block_shift;
-    const int32_t slot = a.slots[row];
-    if (slot < 0) return;
-    if (uint32_t(slot) >= a.total_slots) {
-        if (lane == 0 && rest == 0 && a.status) atomicOr(a.status, uint32_t(SAETTA_PAGED_BAD_SLOT));
-        return;
-    }
-    const uint32_t block = uint32_t(slot) >> a.block_shift, off = uint32_t(slot) & (B - 1);
-    if (row) {
-        const int32_t prev = a.slots[row - 1];
-        if (prev >= 0 && uint32_t(prev) >> a.block_shift == block) {
-            // not a leader; a row that does not follow its predecessor is not written
-            if (prev + 1 != slot && lane == 0 && rest == 0 && a.status) atomicOr(a.status, uint32_t(SAETTA_PAGED_BAD_SLOT));
-            return;
-        }
-    }
-    // the run: rows at slot, slot + 1, ... within the block
-    uint32_t n = 1;
-    while (true) {
-        const uint32_t r = row + n + lane;
-        const bool in = r < a.rows && off + n + lane < B && a.slots[r] == slot + int32_t(n + lane);
-        const uint32_t ballot = __ballot_sync(0xffffffffu, in);
-        const uint32_t more = ballot == 0xffffffffu ? 32 : uint32_t(__ffs(int(~ballot)) - 1);
-        n += more;
-        if (more < 32) break;
+    pdl_wait();
+    uint32_t leads, follows; // of the 16 rows
+    int32_t slot = -1;
+    {
+        const uint32_t row = row0 + lane;
+        const bool in = lane < 16 && row < a.rows;
+        slot = in ? a.slots[row] : -1;
+        const int32_t prev = in && row ? a.slots[row - 1] : -1;
+        const bool real = slot >= 0 && uint32_t(slot) < a.total_slots;
+        const bool same = real && prev >= 0 && uint32_t(prev) >> a.block_shift == uint32_t(slot) >> a.block_shift;
+        leads = __ballot_sync(0xffffffffu, real && !same);
+        follows = __ballot_sync(0xffffffffu, same && prev + 1 == slot);
+        // a slot outside the cache, or one that does not follow its predecessor in the same block
+        const bool bad = slot >= 0 && (!real || (same && prev + 1 != slot));
+        if (rest == 0 && warp == 0 && bad && a.status) atomicOr(a.status, uint32_t(SAETTA_PAGED_BAD_SLOT));
     }
     const void *x = side ? a.v : a.k;
     const size_t stride = side ? a.v_stride : a.k_stride;
     const uint32_t sub = lane / kLanes, col = (lane % kLanes) * 8;
-    const size_t x0 = size_t(row) * stride + size_t(head) * D + col;
-    float amax = 0.f;
-    for (uint32_t i = sub; i < n; i += kRows) {
-        float f[8];
-        load8<DT>(x, x0 + size_t(i) * stride, f);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float m = fabsf(f[j]);
-            amax = m < INFINITY ? fmaxf(amax, m) : amax; // an infinity saturates, a NaN stays one: neither places the range
+    uint32_t turn = 0; // whose short run is next
+    for (; leads; leads &= leads - 1) {
+        const uint32_t k = uint32_t(__ffs(int(leads)) - 1), row = row0 + k;
+        const uint32_t first = uint32_t(__shfl_sync(0xffffffffu, slot, k)), block = first >> a.block_shift, off = first & (B - 1);
+        uint32_t n = 1 + uint32_t(__ffs(int(~(follows >> (k + 1)))) - 1); // rows of the run, within these 16
+        while (k + n >= 16) { // and behind them
+            const uint32_t r = row + n + lane;
+            const uint32_t ballot = __ballot_sync(0xffffffffu, r < a.rows && off + n + lane < B && a.slots[r] == int32_t(first + n + lane));
+            const uint32_t more = ballot == 0xffffffffu ? 32 : uint32_t(__ffs(int(~ballot)) - 1);
+            n += more;
+            if (more < 32) break;
         }
-    }
+        const bool wide = n > 2 * kRows; // all warps take part
+        if (!wide && turn++ % 8 != warp) continue;
+        const uint32_t i0 = (wide ? warp * kRows : 0) + sub, di = wide ? 8 * kRows : kRows;
+        const size_t x0 = size_t(row) * stride + size_t(head) * D + col;
+        float amax = 0.f;
+#pragma unroll 4
+        for (uint32_t i = i0; i < n; i += di) {
+            float f[8];
+            load8<DT>(x, x0 + size_t(i) * stride, f);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    float *sp = a.scales + (size_t(block) * a.kv_heads + head) * 2 + side;
-    uint8_t *page = (side ? a.values : a.keys) + (size_t(block) * a.kv_heads + head) * B * D;
-    float scale = pow2_scale(amax);
-    if (off) { // a block that goes on: its scale never falls, and what it holds follows it
-        const float was = *sp;
-        scale = fmaxf(scale, was);
-        if (scale != was) {
+            for (int j = 0; j < 8; j++) {
+                const float m = fabsf(f[j]);
+                amax = m < INFINITY ? fmaxf(amax, m) : amax; // an infinity saturates, a NaN stays one: neither places the range
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        float *sp = a.scales + (size_t(block) * a.kv_heads + head) * 2 + side;
+        const float was = off ? *sp : 0.f;
+        if (wide) {
+            if (lane == 0) red[warp] = amax;
+            __syncthreads(); // (and `was` has been read)
+#pragma unroll
+            for (int w = 0; w < 8; w++) amax = fmaxf(amax, red[w]);
+        }
+        uint8_t *page = (side ? a.values : a.keys) + (size_t(block) * a.kv_heads + head) * B * D;
+        const float fresh = pow2_scale(amax), scale = off ? fmaxf(fresh, was) : fresh;
+        if (off && scale != was) { // a block that goes on: its scale never falls, and what it holds follows it
             const float f = was / scale;
-            for (uint32_t i = lane; i < off * D / 8; i += 32) {
+            for (uint32_t i = wide ? threadIdx.x : lane; i < off * D / 8; i += wide ? 256 : 32) {
                 uint2 *p = reinterpret_cast<uint2 *>(page) + i;
                 uint2 w = *p;
 #pragma unroll
@@ -296,17 +306,18 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
                 *p = w;
             }
         }
-    }
-    __syncwarp();
-    if (lane == 0) *sp = scale;
-    const float inv = 1.f / scale;
-    for (uint32_t i = sub; i < n; i += kRows) {
-        float f[8];
-        load8<DT>(x, x0 + size_t(i) * stride, f);
-        uint2 w;
-        w.x = e4m3x2(f[0] * inv, f[1] * inv) | e4m3x2(f[2] * inv, f[3] * inv) << 16;
-        w.y = e4m3x2(f[4] * inv, f[5] * inv) | e4m3x2(f[6] * inv, f[7] * inv) << 16;
-        *reinterpret_cast<uint2 *>(page + size_t(off + i) * D + col) = w;
+        if (lane == 0 && (!wide || warp == 0)) *sp = scale;
+        const float inv = 1.f / scale;
+#pragma unroll 4
+        for (uint32_t i = i0; i < n; i += di) {
+            float f[8];
+            load8<DT>(x, x0 + size_t(i) * stride, f);
+            uint2 w;
+            w.x = e4m3x2(f[0] * inv, f[1] * inv) | e4m3x2(f[2] * inv, f[3] * inv) << 16;
+            w.y = e4m3x2(f[4] * inv, f[5] * inv) | e4m3x2(f[6] * inv, f[7] * inv) << 16;
+            *reinterpret_cast<uint2 *>(page + size_t(off + i) * D + col) = w;
+        }
+        if (wide) __syncthreads(); // `red` may be written again
     }
 }
 
@@ -435,7 +446,7 @@ int saetta_paged_assign(int device, size_t seqs, size_t block_tokens, const uint
                        slots_dev, positions_dev, kv_lens_out_dev, free_count_out_dev, status_dev, uint32_t(seqs), uint32_t(table_stride),
                        uint32_t(shift), uint32_t(free_cap), uint32_t(rows_cap)};
     const size_t smem = 4 * (seqs + 1) * sizeof(uint32_t);
-    SAETTA_CUDA(cudaFuncSetAttribute(paged_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(4 * (kPagedMaxSeqs + 1) * 4)));
+    if (smem > 48 * 1024) SAETTA_CUDA(cudaFuncSetAttribute(paged_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(4 * (kPagedMaxSeqs + 1) * 4)));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     const unsigned ctas = rows_cap > 4096 ? 8 : 1;
@@ -464,11 +475,11 @@ int saetta_paged_store(saetta_paged_cache *c, const void *k_dev, const void *v_d
     if (!guard.ok) return fail(SAETTA_ERR_CUDA, "paged store: cannot select the device");
     const StoreArgs a{k_dev, v_dev, slots_dev, c->keys, c->values, c->scales, status_dev, k_stride, v_stride, uint32_t(rows),
                       uint32_t(c->kv_heads), uint32_t(block_shift(c->block_tokens)), uint32_t(c->blocks * c->block_tokens)};
-    const size_t units = rows * c->kv_heads * 2;
+    const size_t ctas = (rows + 15) / 16 * c->kv_heads * 2;
     void (*kernel)(StoreArgs) = nullptr;
     if (c->head_dim == 256) kernel = dtype == SAETTA_F32 ? paged_store_kernel<SAETTA_F32, 256> : dtype == SAETTA_F16 ? paged_store_kernel<SAETTA_F16, 256> : paged_store_kernel<SAETTA_BF16, 256>;
     else kernel = dtype == SAETTA_F32 ? paged_store_kernel<SAETTA_F32, 128> : dtype == SAETTA_F16 ? paged_store_kernel<SAETTA_F16, 128> : paged_store_kernel<SAETTA_BF16, 128>;
-    SAETTA_CUDA(launch_pdl(kernel, dim3(unsigned((units + 7) / 8)), dim3(256), 0, cudaStream_t(stream), a));
+    SAETTA_CUDA(launch_pdl(kernel, dim3(unsigned(ctas)), dim3(256), 0, cudaStream_t(stream), a));
     return SAETTA_OK;
 }
 

@@ -30,6 +30,7 @@ constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the va
 // spare.  (With each row following for itself past 2 doublings, some row of a CTA did so in every other tile of a random prompt of 8192 keys,
 // and the products wait for it; now in one of ten.)
 constexpr float kPpShift = 5.5f, kPpHalf = -8.f /* see split_weights */, kPpRescale = 3.f, kPpSpare = 0.5f;
+constexpr uint32_t kPpGroup = 8;  // parts of an item that one CTA joins by itself
 constexpr int kPpScaleRing = 4, kPpScales = 9;
 
 // What the roles of a CTA need of an item: one warp walks the items and leaves this in a small ring of shared memory.  (With a walk in
@@ -228,8 +229,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     uint64_t *k_full = bars, *v_full = k_full + NK, *k_empty = v_full + NV, *v_empty = k_empty + NK, *sc_full = v_empty + NV, *sc_empty = sc_full + kPpScaleRing,
              *item_full = sc_empty + kPpScaleRing, *item_empty = item_full + kPpItems,
              *s_full = item_empty + kPpItems /* one for each team: a wait by parity must not find the other's phase */, *p_full = s_full + 2,
-             *pv_done = p_full + 2, *q_full = pv_done + 2, *q_empty = q_full + 1, *s_free = q_full + 2, *o_final = q_full + 3, *o_empty = q_full + 4,
-             *all_met = q_full + 5, *x_met = q_full + 6 /* [4 tiles][4 row quarters] */;
+             *pv_done = p_full + 2, *q_full = pv_done + 2, *q_empty = q_full + 1, *s_free = q_full + 2, *o_final = s_free + 1, *o_empty = s_free + 2,
+             *all_met = s_free + 3, *x_met = s_free + 4 /* [4 tiles][4 row quarters] */;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(x_met + 16);
     volatile uint32_t *never_set = tmem_slot + 1, *arrived = tmem_slot + 2;
     uint8_t *row_e = reinterpret_cast<uint8_t *>(tmem_slot + 4); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
@@ -700,53 +701,80 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             if (parts > 1) {
                 if (cq == 0) *reinterpret_cast<float2 *>(part + kPpRows * D + row * 2) = make_float2(m, l);
                 if (warp == 0 && lane == 0) part[kPpRows * (D + 2)] = vref;
-                // the last CTA of the item to arrive joins the parts, in the order of the CTAs
-                __threadfence();
-                PP_MEET_ALL();
-                if (warp == 0 && lane == 0) {
-                    uint32_t *counter = a.words + kPagedCounters + c0;
-                    const uint32_t n = atomicAdd(counter, 1);
-                    if (n + 1 == parts) *counter = 0;
-                    *arrived = n + 1;
+                // The parts are joined by the last CTA to arrive, in the order of the CTAs; many of them in two rounds, groups of some first.
+                uint32_t per = parts;
+                if (parts > kPpGroup) {
+                    per = 2;
+                    while (per * per < parts) per++;
                 }
-                PP_MEET_ALL();
-                const bool last = *arrived == parts;
-                PP_MEET_ALL(); // `arrived` has been read
-                if (last && live) {
-                    __threadfence();
-                    auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + p) * 2 + (p == 0 ? 1 : 0)) * a.part_floats; };
-                    float top = -INFINITY, sum = 0.f;
-                    #pragma unroll 1
-                    for (uint32_t p = 0; p < parts; p++) top = fmaxf(top, __ldcg(part_of(p) + kPpRows * D + row * 2));
-                    const float mu = top == -INFINITY ? 0.f : top;
-                    float vtop = 0.f;
+                const uint32_t groups = (parts + per - 1) / per, mine = (blockIdx.x - c0) / per;
+                uint32_t lo = mine * per, step = 1, n = min(per, parts - lo);
+                // a group's counter: by its first CTA, which may begin another item's tail as well
+                uint32_t *counter = a.words + kPagedCounters + (mine ? gridDim.x : 0) + c0 + lo;
+                auto part_of = [&](uint32_t p) { return a.parts + (size_t(c0 + lo + p * step) * 2 + (lo + p * step == 0 ? 1 : 0)) * a.part_floats; };
 #pragma unroll 1
-                    for (uint32_t p = 0; p < parts; p++) vtop = fmaxf(vtop, __ldcg(part_of(p) + kPpRows * (D + 2)));
-#pragma unroll 1
-                    for (uint32_t p = 0; p < parts; p++) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(p) + kPpRows * D + row * 2));
-                        sum += ml.y * ex2_approx(ml.x - mu);
+                for (bool last = groups == 1;; last = true) {
+                    PP_MEET_ALL();
+                    if (warp == 0 && lane == 0) {
+                        __threadfence(); // (the others' writes too: they came before the meeting)
+                        const uint32_t k = atomicAdd(counter, 1) + 1;
+                        if (k == n) *counter = 0;
+                        __threadfence();
+                        *arrived = k;
                     }
-                    const float is = inverse(sum) * vtop;
+                    PP_MEET_ALL();
+                    const bool mine_to_do = *arrived == n;
+                    PP_MEET_ALL(); // `arrived` has been read
+                    if (!mine_to_do) break;
+                    // each row's maximum and sum; the weights take the place of the parts' maxima
+                    float top = -INFINITY, sum = 0.f, vtop = 0.f;
+                    if (cq == 0 && live) {
+#pragma unroll 4
+                        for (uint32_t p = 0; p < n; p++) {
+                            top = fmaxf(top, __ldcg(part_of(p) + kPpRows * D + row * 2));
+                            vtop = fmaxf(vtop, __ldcg(part_of(p) + kPpRows * (D + 2)));
+                        }
+                        const float mu = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+                        for (uint32_t p = 0; p < n; p++) {
+                            float2 *ml = reinterpret_cast<float2 *>(part_of(p) + kPpRows * D + row * 2);
+                            const float2 x = __ldcg(ml);
+                            const float w = ex2_approx(x.x - mu);
+                            sum = fmaf(x.y, w, sum);
+                            __stcg(&ml->x, w * (__ldcg(part_of(p) + kPpRows * (D + 2)) / vtop));
+                        }
+                        lx[row] = inverse(sum) * vtop;
+                        __threadfence();
+                    }
+                    PP_MEET_ALL();
+                    if (live) {
+                        const float is = lx[row];
 #pragma unroll 1
-                    for (int k = 0; k < D / 4; k += 16) {
-                        const int d = cq * (D / 4) + k;
-                        float4 v[4];
+                        for (int k = 0; k < D / 4; k += 8) {
+                            const int d = cq * (D / 4) + k;
+                            float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+                            for (uint32_t p = 0; p < n; p++) {
+                                const float *pp = part_of(p);
+                                const float wt = __ldcg(pp + kPpRows * D + row * 2);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-                        for (uint32_t p = 0; p < parts; p++) {
-                            const float *pp = part_of(p);
-                            const float wt = ex2_approx(__ldcg(pp + kPpRows * D + row * 2) - mu) * (__ldcg(pp + kPpRows * (D + 2)) / vtop);
+                                for (int j = 0; j < 2; j++) {
+                                    const float4 u = __ldcg(reinterpret_cast<const float4 *>(pp + size_t(row) * D + d + 4 * j));
+                                    v[j].x = fmaf(u.x, wt, v[j].x), v[j].y = fmaf(u.y, wt, v[j].y), v[j].z = fmaf(u.z, wt, v[j].z), v[j].w = fmaf(u.w, wt, v[j].w);
+                                }
+                            }
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const float4 u = __ldcg(reinterpret_cast<const float4 *>(pp + size_t(row) * D + d + 4 * j));
-                                v[j].x = fmaf(u.x, wt, v[j].x), v[j].y = fmaf(u.y, wt, v[j].y), v[j].z = fmaf(u.z, wt, v[j].z), v[j].w = fmaf(u.w, wt, v[j].w);
+                            for (int j = 0; j < 2; j++) {
+                                if (last) finish(d + 4 * j, v[j], is);
+                                else *reinterpret_cast<float4 *>(part_of(0) + size_t(row) * D + d + 4 * j) = v[j];
                             }
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; j++) finish(d + 4 * j, v[j], is);
                     }
+                    if (last) break;
+                    PP_MEET_ALL(); // the weights have been read
+                    if (cq == 0 && live) *reinterpret_cast<float2 *>(part_of(0) + kPpRows * D + row * 2) = make_float2(top, sum);
+                    if (warp == 0 && lane == 0) part_of(0)[kPpRows * (D + 2)] = vtop; // (row 0 is always live)
+                    lo = 0, step = per, n = groups, counter = a.words + kPagedCounters + 2 * gridDim.x + c0;
                 }
             }
         }
