@@ -200,21 +200,26 @@ def _check(rc):
 
 def ptr(x):
     """Device (or host) address of a torch tensor, numpy array, ctypes object or int."""
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
+    try:
         return x.data_ptr()
+    except AttributeError:
+        pass
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     return C.addressof(x)
 
 
+_current_stream = None
+
+
 def _stream(stream):
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        global _current_stream
+        if _current_stream is None:
+            from torch.cuda import current_stream as _current_stream
+        return _current_stream().cuda_stream
     return getattr(stream, "cuda_stream", stream)
 
 

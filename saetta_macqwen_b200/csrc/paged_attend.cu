@@ -42,7 +42,7 @@ struct PdLayout {
     static constexpr int kRow = 128 + 4;                      // floats of one row of the exchange buffer
     static constexpr int kExchange = 8 * 8 * kRow * 4;        // 8 warps x 8 rows of 128 dims
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * kPages * 8 /*scales*/ + 3072 /*barriers, items, statistics*/;
+    static constexpr int kSmem = 1024 + kRing + kExchange + kStages * kPages * 8 /*scales*/ + 3 * 1024 /*barriers, items, statistics*/;
 };
 static_assert(PdLayout<256, 2>::kSmem <= 227 * 1024 && PdLayout<128, 2>::kSmem <= 227 * 1024, "fits a CTA's shared memory");
 

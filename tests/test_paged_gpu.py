@@ -382,3 +382,249 @@ def test_many_sequences_in_one_call():
     c.record(op)  # the same call again gives the same bits
     c.check()
     assert (first == c.out).all()
+
+
+def test_rows_of_q_with_a_stride():
+    import torch
+
+    c = Case(16, 2, 256, 32, [(90, 1), (300, 1)], sa.BF16, sa.BF16, seed=3)
+    wide = torch.zeros((2, 16 * 256 + 264), dtype=torch.bfloat16, device="cuda")
+    wide[:, 8:8 + 4096] = c.dev[0].reshape(2, -1)
+    op = c.op()
+    c.record(op, q=wide.data_ptr() + 16, q_stride=wide.shape[1])
+    c.check()
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_value_scales_of_every_size(rows):
+    """Blocks of zeros (their scale is the smallest) beside ordinary ones, and sequences whose values are all tiny or all huge."""
+    import torch
+
+    for kind in range(3):
+        c = Case(16, 2, 256, 16, [(200, rows), (90, rows)], sa.BF16, sa.F32, seed=kind)
+        if kind == 0:
+            for b in c.tables[0, ::3][:3]:
+                c.p.codes[1][b] = 0
+                c.p.scales[b, :, 1] = 2.0 ** -126
+        else:
+            c.p.scales[..., 1] *= 2.0 ** (-100 if kind == 1 else 60)
+        c.p.values.copy_(torch.from_numpy(np.where(np.isnan(TABLE[c.p.values.cpu().numpy()]), 0x7F, c.p.codes[1])))
+        c.p.sc.copy_(torch.from_numpy(c.p.scales.astype(np.float32)))
+        op = c.op()
+        c.record(op)
+        c.check()
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+def test_a_table_entry_outside_the_cache_is_reported_and_left_out(rows):
+    import torch
+
+    c = Case(16, 2, 256, 32, [(300, rows)], sa.BF16, sa.BF16, seed=2)
+    hole = 3  # this block's keys take no part: the same as the sequence without them
+    c.dev[4][0, hole] = c.p.blocks + 7
+    op = c.op()
+    c.record(op)
+    torch.cuda.synchronize()
+    assert op.device_status() == 16
+    got = c.out.cpu().double().numpy()
+    q = c.q.double().numpy()
+    k, v = ((TABLE[side[c.tables[0, :10]]] * c.p.scales[c.tables[0, :10], :, i][:, :, None, None]).transpose(1, 0, 2, 3).reshape(2, 320, 256)
+            for i, side in enumerate(c.p.codes))
+    for i in range(rows):
+        seen = np.array([j for j in range(300 - rows + i + 1) if not hole * 32 <= j < hole * 32 + 32])
+        for h in (0, 9):
+            w = k[h // 8][seen] @ q[i, h] * c.scale
+            w = np.exp(w - w.max())
+            want = w @ v[h // 8][seen] / w.sum()
+            assert np.abs(got[i, h] - want).max() < 2.0 ** -7 * np.abs(v[h // 8][seen]).max()  # bfloat16 weights and output, each 2^-8 of the largest value
+
+
+def test_long_prompt_tails_are_joined_in_two_rounds():
+    """Few rows over many keys: an item lies in more CTAs than one joins by itself."""
+    c = Case(8, 1, 128, 128, [(30000, 16)], sa.F16, sa.F32, seed=1)
+    c.max_rows = 64  # the many-rows kernel
+    op = c.op()
+    c.record(op)
+    c.check()
+    c.max_rows = 2
+    c.record(op)
+    c.max_rows = 16  # (which bound holds)
+    first = c.out.clone()
+    c.record(op)
+    c.check()
+    assert op.device_status() == 0 and first.isfinite().all()
+
+
+def test_offsets_beyond_32_bits():
+    import torch
+
+    blocks = (1 << 32) // (2 * 64 * 256) + 9  # 4 GB of keys and a little more
+    cache = sa.PagedKvCache(0, 2, 256, 64, blocks)
+    rng = np.random.default_rng(0)
+    n = 130
+    k, v = (torch.from_numpy(rng.normal(size=(n, 2, 256)).astype(np.float32)) for _ in range(2))
+    table = [blocks - 1, 3, blocks - 2]
+    slots = [table[j // 64] * 64 + j % 64 for j in range(n)]
+    cache.store(k.cuda(), v.cuda(), i32(slots), n)
+    codes = [np.zeros((3, 2, 64, 256), np.uint8) for _ in range(2)]
+    scales = np.full((3, 2, 2), 1.0)
+    ref_store(*codes, scales, k.double().numpy(), v.double().numpy(), list(range(n)), 64)
+    for rows in (1, 3):
+        q = torch.from_numpy(rng.normal(size=(rows, 16, 256)).astype(np.float32)).to(torch.bfloat16)
+        out = torch.zeros((rows, 16, 256), dtype=torch.bfloat16, device="cuda")
+        op = sa.PagedAttention(0, 16, 2, 256)
+        op.record(cache, q.cuda(), sa.BF16, rows, 1, i32([0, rows]), i32([n]), i32([table]), 3, rows, 1 / 16, out, sa.BF16)
+        torch.cuda.synchronize()
+        want, b = ref_attend(q.double().numpy(), *codes, scales, np.array([[0, 1, 2]]), [0, rows], [n], 64, 1 / 16)
+        lim = bound(sa.BF16, sa.BF16, want, b, n, 256, rows * 8 > 16)
+        assert (np.abs(out.cpu().double().numpy() - want) <= lim).all()
+
+
+def test_two_ops_on_two_streams_at_once():
+    import torch
+
+    cases = [Case(16, 2, 256, 64, [(3000, 1), (500, 1)], sa.BF16, sa.BF16, seed=1), Case(16, 2, 256, 64, [(900, 120)], sa.BF16, sa.BF16, seed=2)]
+    ops = [c.op() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, op, s in zip(cases, ops, streams):
+            c.record(op, stream=s)
+    for c, op in zip(cases, ops):
+        c.check()
+        assert op.device_status() == 0
+
+
+# ----------------------------------------------------------------- together
+
+
+class Server:
+    """A small server's buffers: requests of one layer, three launches a step, all lengths on the device."""
+
+    def __init__(self, heads=16, kv=2, dim=256, block=16, blocks=64, seqs=5, width=12, rows_cap=40, seed=0):
+        import torch
+
+        self.rng = np.random.default_rng(seed)
+        self.heads, self.kv, self.dim, self.block, self.seqs, self.width, self.cap = heads, kv, dim, block, seqs, width, rows_cap
+        self.cache = sa.PagedKvCache(0, kv, dim, block, blocks)
+        self.op = sa.PagedAttention(0, heads, kv, dim)
+        self.free = [int(x) for x in self.rng.permutation(blocks)]
+        self.count, self.lens, self.tables = blocks, [0] * seqs, [[-1] * width for _ in range(seqs)]
+        self.codes = [np.zeros((blocks, kv, block, dim), np.uint8) for _ in range(2)]
+        self.scales = np.zeros((blocks, kv, 2))
+        z = lambda *n: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.d = dict(lens=i32(self.lens), new=z(seqs), fin=z(seqs), free=i32(self.free), count=i32([self.count]), tables=i32(self.tables), starts=z(seqs + 1),
+                      slots=z(rows_cap), pos=z(rows_cap), status=z(1), store_status=z(1))
+        self.k, self.v = (torch.zeros((rows_cap, kv, dim), device="cuda") for _ in range(2))
+        self.q = torch.zeros((rows_cap, heads, dim), dtype=torch.bfloat16, device="cuda")
+        self.gate = torch.zeros((rows_cap, heads, 2 * dim), device="cuda")
+        self.out = torch.zeros((rows_cap, heads, dim), dtype=torch.bfloat16, device="cuda")
+
+    def launch(self, max_rows, stream=None):
+        d = self.d
+        sa.paged_assign(0, self.seqs, self.block, d["lens"], d["new"], d["free"], len(self.free), d["count"], d["tables"], self.width, d["starts"], d["slots"], d["pos"],
+                        self.cap, d["lens"], d["count"], d["status"], finished=d["fin"], stream=stream)
+        self.cache.store(self.k, self.v, d["slots"], self.cap, status=d["store_status"], stream=stream)
+        self.op.record(self.cache, self.q, sa.BF16, self.cap, self.seqs, d["starts"], d["lens"], d["tables"], self.width, max_rows, self.dim ** -0.5, self.out, sa.BF16,
+                       q_and_gate=self.gate, stream=stream)
+
+    def feed(self, new, fin):
+        import torch
+
+        self.new, self.fin = new, fin
+        self.d["new"].copy_(i32(new)), self.d["fin"].copy_(i32(fin))
+        for t in (self.k, self.v, self.q, self.gate):
+            t.copy_(torch.from_numpy(self.rng.normal(size=tuple(t.shape)).astype(np.float32)))
+        self.out.fill_(5.0)
+
+    def check(self, max_rows):
+        import torch
+
+        torch.cuda.synchronize()
+        starts, slots, pos, self.lens, self.count = ref_assign(self.lens, self.new, self.fin, self.free, self.count, self.tables, self.block, self.cap)
+        assert self.d["status"].item() == 0 and self.d["store_status"].item() == 0 and self.op.device_status() == 0
+        assert self.d["slots"].cpu().tolist() == slots and self.d["pos"].cpu().tolist() == pos and self.d["tables"].cpu().tolist() == self.tables
+        ref_store(*self.codes, self.scales, self.k.cpu().double().numpy(), self.v.cpu().double().numpy(), slots, self.block)
+        want, b = ref_attend(self.q.cpu().double().numpy(), *self.codes, self.scales, np.array(self.tables), starts, self.lens, self.block, self.dim ** -0.5,
+                             self.gate[..., self.dim:].cpu().double().numpy())
+        got, total = self.out.cpu().double().numpy(), starts[-1]
+        lim = bound(sa.BF16, sa.BF16, want, b, max(self.lens + [1]), self.dim, max_rows * self.heads // self.kv > 16)
+        assert (np.abs(got - want) <= lim)[:total].all() and (got[total:] == 5.0).all()
+
+
+STEPS = [([7, 0, 19, 1, 3], [0] * 5), ([1, 16, 1, 1, 1], [0] * 5), ([1, 1, 1, 1, 1], [0, 0, 0, 1, 0]), ([0, 1, 1, 9, 1], [1, 0, 0, 0, 0]), ([12, 1, 1, 1, 1], [0, 0, 1, 0, 0]),
+         ([1] * 5, [0] * 5), ([0] * 5, [0] * 5), ([0, 2, 0, 0, 1], [1, 0, 0, 0, 0])]
+
+
+def test_steps_of_a_server():
+    srv = Server()
+    for new, fin in STEPS:
+        srv.feed(new, fin)
+        srv.launch(max(new))
+        srv.check(max(new))
+
+
+@pytest.mark.parametrize("max_rows", [2, 19])
+def test_a_recorded_step_serves_other_lengths(max_rows):
+    """One capture replayed for every step, lengths and tables read on the device; more rows than the hint only cost time."""
+    import torch
+
+    srv = Server(seed=max_rows)
+    srv.feed([1] * 5, [0] * 5)
+    srv.launch(max_rows)
+    srv.check(max_rows)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        srv.launch(max_rows)
+    for new, fin in STEPS:
+        srv.feed(new, fin)
+        graph.replay()
+        srv.check(max_rows)
+
+
+def test_a_step_that_does_not_fit_leaves_everything():
+    import torch
+
+    srv = Server(blocks=4)
+    srv.feed([20, 20, 0, 0, 0], [0] * 5)
+    srv.launch(20)
+    srv.check(20)
+    before = srv.d["tables"].clone(), srv.d["lens"].clone(), [t.clone() for t in (srv.out,)]
+    srv.feed([20, 20, 0, 0, 0], [0] * 5)  # two more blocks are needed than there are
+    srv.launch(20)
+    torch.cuda.synchronize()
+    assert srv.d["status"].item() == sa.PAGED_NO_BLOCKS
+    assert (srv.d["tables"] == before[0]).all() and (srv.d["lens"] == before[1]).all()
+    assert (srv.out == 5.0).all() and (srv.d["slots"] == -1).all()
+
+
+def test_prep_paged_step_and_output_projection():
+    """The framework's own layer around the cache: prep's f32 keys and queries in, the projection's f32 input out."""
+    import torch
+
+    H, KV, D, n = 16, 2, 256, 23
+    srv = Server(blocks=8, seqs=1, rows_cap=n, width=4)
+    rng = np.random.default_rng(8)
+    qg, k, v = (torch.from_numpy(rng.normal(size=s).astype(np.float32)).cuda() for s in ((n, H, 2 * D), (n, KV, D), (n, KV, D)))
+    ones = torch.ones(D, device="cuda")
+    q, k_out, out = torch.zeros((n, H, D), device="cuda"), torch.zeros((n, KV, D), device="cuda"), torch.zeros((n, H, D), device="cuda")
+    scratch = sa.GpuKvCache(0, 32, 128)
+    sa.attention_prep(sa.PrepParams(H, KV, D, 64, 1.0e7, 1.0e-6), n, qg, k, v, ones, ones, q, sa.F32, scratch, pos=0, k_out=k_out)
+    d = srv.d
+    d["new"].copy_(i32([n]))
+    sa.paged_assign(0, 1, 16, d["lens"], d["new"], d["free"], 8, d["count"], d["tables"], 4, d["starts"], d["slots"], d["pos"], n, d["lens"], d["count"], d["status"])
+    srv.cache.store(k_out, v, d["slots"], n)
+    srv.op.record(srv.cache, q, sa.F32, n, 1, d["starts"], d["lens"], d["tables"], 4, n, 1 / 16, out, sa.F32, q_and_gate=qg)
+    words = torch.from_numpy(rng.integers(0, 2**31, (64, H * D // 4)).astype(np.int32)).cuda()  # 64 rows of an 8-bit matrix
+    sc, bi = (torch.full((64, H * D // 64), x, dtype=torch.bfloat16, device="cuda") for x in (0.01, -1.28))
+    y = torch.zeros((1, 64), device="cuda")
+    sa.qmv_rows(0, words, sc, bi, 8, 64, H * D, 1, out[n - 1], y)
+    torch.cuda.synchronize()
+    kr, qr = k_out.cpu().double().numpy(), q.cpu().double().numpy()
+    ref_store(*srv.codes, srv.scales, kr, v.cpu().double().numpy(), d["slots"].cpu().tolist(), 16)
+    want, b = ref_attend(qr, *srv.codes, srv.scales, d["tables"].cpu().numpy(), [0, n], [n], 16, 1 / 16, qg[..., D:].cpu().double().numpy())
+    assert (np.abs(out.cpu().double().numpy() - want) <= bound(sa.F32, sa.F32, want, b, n, D, True)).all()
+    w = (words.cpu().numpy().view(np.uint8).astype(np.float64).reshape(64, H * D)) * float(sc[0, 0]) + float(bi[0, 0])
+    row = out[n - 1].cpu().double().numpy().ravel()
+    assert np.abs(y.cpu().double().numpy()[0] - w @ row).max() <= H * D * 2.0 ** -23 * (np.abs(w) @ np.abs(row)).max()
