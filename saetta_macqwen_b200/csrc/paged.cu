@@ -8,6 +8,7 @@
 // src/kv_quant.rs:54-105, in one buffer per sequence).
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -149,18 +150,32 @@ __global__ void __launch_bounds__(kAssignThreads) paged_assign_kernel(const Assi
         const uint32_t have = (len0[s] + B - 1) >> a.block_shift;
         a.tables[size_t(s) * a.table_stride + have + (e - take0[s])] = a.free_blocks[top - 1 - e];
     }
-    for (uint32_t r = gtid; r < a.rows_cap; r += gthreads) {
-        int32_t slot = -1, pos = -1;
-        if (r < rows) {
-            const uint32_t s = last_at_or_below(row0, a.seqs, r);
-            pos = int32_t(len0[s] + (r - row0[s]));
-            const uint32_t have = (len0[s] + B - 1) >> a.block_shift, idx = uint32_t(pos) >> a.block_shift;
+    // Four rows a thread: one search, then along the sequences.
+    const bool quads = (reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) % 16 == 0;
+    for (uint32_t r0 = gtid * 4; r0 < a.rows_cap; r0 += gthreads * 4) {
+        int32_t slot[4], pos[4];
+        uint32_t s = r0 < rows ? last_at_or_below(row0, a.seqs, r0) : 0, end = r0 < rows ? row0[s + 1] : 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const uint32_t r = r0 + j;
+            slot[j] = pos[j] = -1;
+            if (r >= rows) continue;
+            while (r >= end) end = row0[++s + 1];
+            pos[j] = int32_t(len0[s] + (r - row0[s]));
+            const uint32_t have = (len0[s] + B - 1) >> a.block_shift, idx = uint32_t(pos[j]) >> a.block_shift;
             // the block is one the sequence had, or one of those taken above (read from the stack: no wait for the table)
             const int32_t block = idx < have ? a.tables[size_t(s) * a.table_stride + idx] : a.free_blocks[top - 1 - (take0[s] + idx - have)];
-            slot = int32_t((uint32_t(block) << a.block_shift) + (uint32_t(pos) & (B - 1)));
+            slot[j] = int32_t((uint32_t(block) << a.block_shift) + (uint32_t(pos[j]) & (B - 1)));
         }
-        a.slots[r] = slot;
-        if (a.positions) a.positions[r] = pos;
+        if (quads && r0 + 4 <= a.rows_cap) {
+            *reinterpret_cast<int4 *>(a.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            if (a.positions) *reinterpret_cast<int4 *>(a.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+            for (uint32_t j = 0; j < 4 && r0 + j < a.rows_cap; j++) {
+                a.slots[r0 + j] = slot[j];
+                if (a.positions) a.positions[r0 + j] = pos[j];
+            }
+        }
     }
     for (uint32_t s = gtid; s <= a.seqs; s += gthreads) {
         a.row_starts[s] = row0[s];
@@ -495,7 +510,7 @@ int saetta_paged_attention_create(int device, size_t heads, size_t kv_heads, siz
     auto *op = new (std::nothrow) saetta_paged_attention();
     if (!op) return fail(SAETTA_ERR_NO_MEM, "PagedAttention: host allocation");
     op->device = device, op->heads = heads, op->kv_heads = kv_heads, op->head_dim = head_dim;
-    op->ctas = sm_count(device);
+    op->ctas = std::min(sm_count(device), 255); // (paged_cut)
     op->part_floats = 128 * (head_dim + 2) + 4; // 128 rows: the largest tile; (m, l) of each; the value scale O is kept by
     void *p = nullptr, *w = nullptr;
     const size_t words = size_t(kPagedCounters) + 3 * size_t(op->ctas);
@@ -549,7 +564,8 @@ int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *ca
     a.q_dtype = q_dtype, a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
     // which kernel: see kPagedFewRows
-    if (batch.max_rows * a.group <= kPagedFewRows) return launch_paged_decode(a, cache, uint32_t(batch.max_rows * a.group), op->ctas, cudaStream_t(stream));
+    const size_t rows = std::max<size_t>(1, std::min(batch.max_rows, batch.rows)) * a.group;
+    if (rows <= kPagedFewRows) return launch_paged_decode(a, cache, uint32_t(rows), op->ctas, cudaStream_t(stream));
     return launch_paged_prefill(a, cache, op->ctas, cudaStream_t(stream));
 }
 

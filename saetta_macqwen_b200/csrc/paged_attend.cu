@@ -223,7 +223,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = min(max(int(__float_as_uint(top) >> 23), 8), 247) - 134; // 2^(e + 7) <= top < 2^(e + 8)
+            const int e = min(max(int(__float_as_uint(top) >> 23), 8), 254) - 134; // 2^(e + 7) <= top < 2^(e + 8)
             const float up = __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
             for (int c = 0; c < kSlabs * 4; c++) {

@@ -25,11 +25,17 @@ namespace saetta {
 constexpr int kPpRows = 128, kPpKeys = 128, kPpThreads = 768;
 constexpr int kPpWarps = 16;  // of the softmax: two teams of eight, which take the tiles by turns
 constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the values
-// e4m3 ends at 448 = 2^8.8, and its smallest steps should lie low beside the weights: w is kept times 2^5.5, by a maximum that O follows only when a
-// row's scores pass it by 3 doublings (w stays below 2^8.5); then all 32 rows of the warp are brought up to date, with half a doubling to
+// e4m3 ends at 448 = 2^8.8, and its smallest steps should lie low beside the weights: w is kept times 2^6, by a maximum that O follows only when a
+// row's scores pass it by 2.5 doublings (w stays below 2^8.5); then all 32 rows of the warp are brought up to date, with half a doubling to
 // spare.  (With each row following for itself past 2 doublings, some row of a CTA did so in every other tile of a random prompt of 8192 keys,
-// and the products wait for it; now in one of ten.)
-constexpr float kPpShift = 5.5f, kPpHalf = -8.f /* see split_weights */, kPpRescale = 3.f, kPpSpare = 0.5f;
+// and the products wait for it; now in one of ten.)  With three terms the smallest steps, and not the last term's rounding, are what
+// remains: w is kept times 2^8 and the maximum follows past half a doubling.  (Over 7 prompts of up to 3500 keys, against 64 bits: 2^5.5 and 3
+// doublings 0.00046 in 634 us, 2^8 and a half 0.00030 in 653 us; a binary16 output alone is off by 0.00021.)
+template <int PARTS>
+constexpr float kPpShift = PARTS == 3 ? 8.f : 6.f;
+template <int PARTS>
+constexpr float kPpRescale = PARTS == 3 ? 0.5f : 2.5f;
+constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 0.5f;
 constexpr uint32_t kPpGroup = 8;  // parts of an item that one CTA joins by itself
 constexpr int kPpScaleRing = 4, kPpScales = 9;
 
@@ -180,6 +186,7 @@ __device__ __forceinline__ void split(float (&x)[N], uint32_t (&w)[PARTS][N / 4]
 // The same for weights, which are not negative, in a third of the time: they come times 2^-8 (kPpHalf), where the exponent field of a binary16
 // value is that of its e4m3 code, subnormals included, so that the code is the value's bits 14 .. 7.  Each term but the last is cut off there,
 // what remains is exact, and the last is rounded (half up): two terms are off by 2^-8 of the weight at most, three hold the binary16 value.
+// (Rounding the first of two as well, which needs the second's signs, halves that and takes 2 to 4 % longer.)
 template <int PARTS>
 __device__ __forceinline__ void split_weights(const float *x, uint32_t (&w)[PARTS]) { // of four
     uint32_t h0 = pack_half2(x[0], x[1]), h1 = pack_half2(x[2], x[3]);
@@ -470,7 +477,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
             }
             // a power of two brings the row's largest to [128, 256)
-            const int e = min(max(int(__float_as_uint(top) >> 23), 8), 247) - 134;
+            const int e = min(max(int(__float_as_uint(top) >> 23), 8), 254) - 134;
             const float up = __uint_as_float(uint32_t(127 - e) << 23);
             // the products of the tile before have read the old Q, and its softmax the old factors
             PP_WAIT(q_empty, (ni & 1) ^ 1);
@@ -489,7 +496,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     }
                     uint32_t w[PARTS][2];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] *= up;
+                    for (int k = 0; k < 8; k++) x[k] = fmaf(x[k], up, x[k] * 0.f); // (an infinity becomes NaN: e4m3 has none)
                     split<PARTS, 8>(x, w);
 #pragma unroll
                     for (int p = 0; p < PARTS; p++) *reinterpret_cast<uint2 *>(dst + p * L::kQPart + 8 * h) = make_uint2(w[p][0], w[p][1]);
@@ -523,7 +530,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             float m = -INFINITY, l = 0.f;
             // The running maximum after a tile whose own is `top` (the same in all four warps that share the rows).
             auto follow = [&](float was, float top) {
-                const bool need = __any_sync(0xffffffffu, top > was + kPpRescale);
+                const bool need = __any_sync(0xffffffffu, top > was + kPpRescale<PARTS>);
                 return need ? fmaxf(was, __bfloat162float(__float2bfloat16_ru(top + kPpSpare))) : was;
             };
             for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
@@ -555,7 +562,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     const float *x = reinterpret_cast<const float *>(&s[b >> 1][(b & 1) * 16]);
                     float t[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
                     t[0] = max3(t[0], x[6], x[7]), t[1] = max3(t[1], x[8], x[9]), t[0] = max3(t[0], x[10], x[11]), t[1] = max3(t[1], x[12], x[13]);
-                    mx = fmaxf(mx, fmaxf(max3(t[0], x[14], x[15]), t[1]) * (fabsf(f) * rs));
+                    mx = fmaxf(mx, fmaxf(max3(t[0], x[14], x[15]), t[1]) * fmaxf(fabsf(f) * rs, FLT_MIN)); // (not 0: that times a masked key's -infinity is NaN)
                 }
                 // The two threads of a row agree on one maximum (rounded up it is still one that no score passes).  Every warp follows the running
                 // maximum through all tiles: the other team's tile first, then its own.  (Waiting for the other team's tile also shows
@@ -597,7 +604,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     }
                     tmem_wait_st();
                 }
-                const float base = kPpShift + kPpHalf - (m == -INFINITY ? 0.f : m);
+                const float base = kPpShift<PARTS> + kPpHalf - (m == -INFINITY ? 0.f : m);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int h = 0; h < 3; h++) {
@@ -608,7 +615,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                         if (h < 2) {
                             float *e = reinterpret_cast<float *>(&s[h][q * 4]);
                             const float2 f = sc[h * 2 + (q >> 2)];
-                            const float c = fabsf(f.x) * rs, d = f.y + base;
+                            const float c = fmaxf(fabsf(f.x) * rs, FLT_MIN), d = f.y + base;
                             const float2 t0 = fma2(make_float2(e[0], e[1]), make_float2(c, c), make_float2(d, d));
                             const float2 t1 = fma2(make_float2(e[2], e[3]), make_float2(c, c), make_float2(d, d));
                             e[0] = ex2_approx(t0.x), e[1] = ex2_approx(t0.y), e[2] = ex2_approx(t1.x), e[3] = ex2_approx(t1.y);

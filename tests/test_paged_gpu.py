@@ -628,3 +628,65 @@ def test_prep_paged_step_and_output_projection():
     w = (words.cpu().numpy().view(np.uint8).astype(np.float64).reshape(64, H * D)) * float(sc[0, 0]) + float(bi[0, 0])
     row = out[n - 1].cpu().double().numpy().ravel()
     assert np.abs(y.cpu().double().numpy()[0] - w @ row).max() <= H * D * 2.0 ** -23 * (np.abs(w) @ np.abs(row)).max()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_queries_of_every_size(rows):
+    """Rows of q near the largest value, with keys that bring the scores back; an infinite and a NaN row, which reach no other."""
+    import torch
+
+    c = Case(16, 2, 256, 32, [(150, rows)], sa.BF16, sa.BF16, seed=6)
+    c.q[:, 1] *= 2.0 ** 124
+    c.q[:, 2] *= 2.0 ** -90
+    c.p.scales[:, 0, 0] *= 2.0 ** -110
+    c.p.sc.copy_(torch.from_numpy(c.p.scales.astype(np.float32)))
+    c.scale = 2.0 ** -18  # of head 1 alone do the scores count
+    clean = c.q.clone()
+    clean[:, 12:14] = 0
+    c.q[:, 12, 7], c.q[:, 13, 200] = float("inf"), float("nan")
+    op = c.op()
+    c.record(op, q=c.q.cuda())
+    torch.cuda.synchronize()
+    got = c.out.cpu().double().numpy()
+    want, b = ref_attend(clean.double().numpy(), *c.p.codes, c.p.scales, c.tables, c.starts, c.kv_lens, c.block, c.scale)
+    lim = bound(sa.BF16, sa.BF16, want, b, 150, 256, rows * 8 > 16)
+    assert np.isnan(got[:, 12:14]).all()
+    keep = [h for h in range(16) if h not in (12, 13)]
+    assert (np.abs(got - want) <= lim)[:, keep].all() and op.device_status() == 0
+
+
+@pytest.mark.parametrize("hint", [0, 1])
+def test_a_hint_below_the_rows_costs_time_alone(hint):
+    for heads, dim in ((16, 128), (9, 256)):
+        c = Case(heads, 1, dim, 16, [(70, 5), (33, 1)], sa.F16, sa.F32, seed=heads)
+        op = c.op()
+        c.max_rows = hint
+        c.record(op)
+        c.max_rows = 1
+        c.check()
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_assign_rows_at_any_address(shift):
+    """slots and positions need no more than 4-byte alignment; runs of every length, and empty ones, side by side."""
+    import torch
+
+    rng = np.random.default_rng(shift)
+    lens, new = [int(x) for x in rng.integers(0, 40, 300)], [int(x) for x in rng.integers(0, 7, 300)]
+    tables = [[-1] * 4 for _ in lens]
+    free = [int(x) for x in rng.permutation(1500)]
+    count = len(free)
+    for s, n in enumerate(lens):
+        for j in range((n + 15) // 16):
+            count -= 1
+            tables[s][j] = free[count]
+    cap = sum(new) + 3
+    z = lambda *n: torch.full(n, 77, dtype=torch.int32, device="cuda")  # noqa: E731
+    d = [i32(x) for x in (lens, new, free, [count], tables)]
+    starts, slots, pos, status = z(301), z(cap + 2), z(cap + 2), z(1)
+    sa.paged_assign(0, 300, 16, d[0], d[1], d[2], 1500, d[3], d[4], 4, starts, slots[shift:], pos[shift:], cap, d[0], d[3], status)
+    torch.cuda.synchronize()
+    w_starts, w_slots, w_pos, w_lens, w_count = ref_assign(lens, new, [0] * 300, free, count, tables, 16, cap)
+    assert starts.cpu().tolist() == w_starts and d[0].cpu().tolist() == w_lens and d[3].item() == w_count and d[4].cpu().tolist() == tables
+    for got, want in ((slots, w_slots), (pos, w_pos)):
+        assert got.cpu().tolist() == [77] * shift + want + [77] * (2 - shift)
