@@ -583,7 +583,9 @@ void saetta_paged_attention_destroy(saetta_paged_attention *op);
  * [rows][heads][head_dim], q_stride values between rows (at least heads * head_dim), rows
  * 16-byte aligned; q_dtype and out_dtype each SAETTA_F32, SAETTA_F16 or SAETTA_BF16.
  * Scores, sums and accumulators are f32; the products take q with the precision of its type,
- * 11 bits of an f32 one, and the probabilities with 11 bits (8 for long bfloat16 chunks). */
+ * 11 bits of an f32 one, and the probabilities with 11 bits; with more than 16 rows (tokens x
+ * heads of a kv head) and bfloat16 q with 8, and down to 2^-15 of the row's largest.  A row of q
+ * with an infinity or a NaN gets NaN.  max_rows below the real count costs time alone. */
 int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *cache,
                         saetta_paged_batch batch, const void *q_dev, int q_dtype, size_t q_stride,
                         const float *q_and_gate_dev, void *out_dev, int out_dtype, float scale,

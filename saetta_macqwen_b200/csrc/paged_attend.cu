@@ -18,6 +18,11 @@
 //  * P is rounded to binary16 (11 bits; p times the value scale relative to the largest of the warp's so far), scores, sums
 //    and accumulators are f32.  Queries enter as binary16 after a power of two for each row, so bfloat16's range
 //    fits; f32 queries are rounded to 11 bits there.
+//
+// Measured: one sequence of 131072 keys (bfloat16, 16 query and 2 kv heads of 256) 40 us (3.4 TB/s; the bytes alone take 20.5), 61 sequences of up to
+// 8192 keys (binary16, 32 over 8 heads of 128) 128 us (3.7 TB/s), 701 keys 12.9 us.  What is left beyond the bytes is the start of a CTA (its share, the
+// first pages, the first bytes: 6 us), the change of items, and the parts' joining (3 to 4 us a round).  (One warp for keys, values and scales together: 61 sequences 139 us; copies issued page
+// by page from one lane: 173; scores of two products for 32 rows in place of the many-rows kernel: 138 against 96.)
 #include <algorithm>
 
 #include "paged_sched.cuh"
@@ -25,7 +30,7 @@
 
 namespace saetta {
 
-constexpr int kPdThreads = 384;  // 8 consumer warps, the producer's group of 4 (one of them works)
+constexpr int kPdThreads = 384;  // 8 consumer warps; items and keys, values, scales; one warp that makes up the group of 4
 constexpr uint32_t kPdGroup = 12; // parts of an item that one CTA joins by itself
 constexpr float kPdRescale = 8.f; // the accumulators follow the running maximum only past this many doublings
 

@@ -13,7 +13,15 @@
 //
 // A tile is 128 rows: `tpt` tokens x the query heads of one kv head.  Key tiles are 128 keys.  Bound by the tensor pipe: 2 * PARTS *
 // 128 * 128 * D multiply-adds for each tile at 8192 a clock and SM.  Roles: sixteen softmax warps in two teams that take
-// tiles by turns (two threads for each row, 64 keys each), four warps that bring a tile's Q rows, one warp each for the K/V copies, the products and the scales.
+// tiles by turns (two threads for each row, 64 keys each), four warps that bring a tile's Q rows, one warp each for the K/V copies, the score
+// products, the scales and the value products.
+//
+// Measured (bfloat16, 16 query and 2 kv heads of 256, 4096 rows at 28672 keys): 1.53 to 1.6 ms in a burst (1.3 PFLOP/s counted as 16-bit
+// products), 1.78 in a stream of calls under the power limit.  With head dim 128 a tile has half the products and the same softmax, which then bounds it: a warp needs 5000
+// clocks for its tile, two teams so 2600 a tile (1024 of products); binary16 queries 3600 (1536).  7 prompts of 425 to 2554 keys, 32 over 8
+// heads of 128, binary16: 653 us.  Beside the tiles: 14,000 clocks before a CTA's first item (its code and share come cold), 10,000 for the first Q rows (later
+// ones come under the tiles before), 12,000 between items, up to 24,000 where the last CTA joins an item's parts.  (A second Q buffer, tried
+// for head dim 128: 688 us against 640.  Q rows four at a time, each read by 8 lanes: 900, from spills.)
 #include <algorithm>
 #include <cfloat>
 
@@ -512,8 +520,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         // Two teams of eight warps take the tiles by turns, so that one team's loads, maxima and hand-overs run under the other's exponentials
         // and the products.  A team takes its 128 x 128 scores into registers at once, which frees their place for the next tile's.  What a
         // tile needs of the one before it is only the running maximum.
-        // (Measured at 4096 rows by 32768 keys: one tile at a time by eight warps 2.25 ms, by sixteen 2.2; two teams with the scores left in
-        // tensor memory, the weights written over them: 1.94, the two teams in step and the products between them.)
+        // (At 4096 rows by 32768 keys, when it was tried: one tile at a time by eight warps 2.25 ms, by sixteen 2.2; two teams with the scores left in
+        // tensor memory, the weights written over them: 1.94, the two teams in step and the products between them; as it is: 1.55.)
         const uint32_t quarter = warp & 3, half = warp >> 2 & 1, team = warp >> 3, row = quarter * 32 + lane;
         const uint32_t lane_addr = (quarter * 32) << 16;
         uint32_t g = 0, all = 0; // tiles, meetings of all warps, so far

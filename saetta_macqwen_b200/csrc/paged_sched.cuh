@@ -118,7 +118,7 @@ struct PagedWalk {
                 head = 0;
                 if (at < end)
                     do q = paged_seq(a, ++seq);
-                    while (!q.n);
+                    while (!q.n && seq + 1 < a.seqs);
                 rtiles = tiles.row_tiles(q);
             }
         }

@@ -690,3 +690,22 @@ def test_assign_rows_at_any_address(shift):
     assert starts.cpu().tolist() == w_starts and d[0].cpu().tolist() == w_lens and d[3].item() == w_count and d[4].cpu().tolist() == tables
     for got, want in ((slots, w_slots), (pos, w_pos)):
         assert got.cpu().tolist() == [77] * shift + want + [77] * (2 - shift)
+
+
+def test_a_plan_of_a_serving_step():
+    """The framework's recorder: three kernels, run again for other lengths."""
+    import torch
+
+    srv = Server(seed=4)
+    plan = sa.Plan(0)
+    torch.cuda.synchronize()
+    with plan.recording():
+        srv.launch(1, stream=plan.stream)
+    assert len(plan) == 3 and "paged_assign" in plan.kernels()[0][0]
+    for new, fin in STEPS:
+        srv.feed(new, fin)
+        torch.cuda.synchronize()
+        plan.set_params(0, 0)
+        plan.run()
+        torch.cuda.synchronize()
+        srv.check(1)
