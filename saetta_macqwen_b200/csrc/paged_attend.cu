@@ -42,6 +42,9 @@ struct PdLayout {
     static constexpr int kSide = kTile * D;
     static constexpr int kStage = 2 * kSide;       // 32 KB
     static constexpr int kStages = 5;
+    // Barriers of landed tiles, two for each stage.  The teams take tiles by turns and the stages are odd in number, so a stage goes from team to team: on
+    // one barrier a team would see every other phase, always of one parity, and take an older use of its own for the tile it waits for.
+    static constexpr int kFull = 2 * kStages;
     static constexpr int kPages = kTile / 16;      // of a tile, at most
     static_assert(kRows * D / 4 >= 256, "every consumer has values to join");
     static constexpr int kRow = 128 + 4;                      // floats of one row of the exchange buffer
@@ -100,7 +103,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *xch = reinterpret_cast<float *>(ring + L::kRing);                  // [8 warps][8 rows][kRow]
     float2 *scl = reinterpret_cast<float2 *>(ring + L::kRing + L::kExchange); // [stage][page]
-    uint64_t *full = reinterpret_cast<uint64_t *>(scl + L::kStages * L::kPages), *empty = full + L::kStages;
+    uint64_t *full = reinterpret_cast<uint64_t *>(scl + L::kStages * L::kPages), *empty = full + L::kFull;
     uint64_t *item_full = empty + L::kStages, *item_empty = item_full + kPdItems;
     uint64_t *scratch = item_empty + kPdItems; // 40 words
     PagedShare *share = reinterpret_cast<PagedShare *>(scratch + 40);
@@ -113,7 +116,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int s = 0; s < L::kStages; s++) mbar_init(&full[s], 34), mbar_init(&empty[s], 4);
+        for (int s = 0; s < L::kFull; s++) mbar_init(&full[s], 34);
+        for (int s = 0; s < L::kStages; s++) mbar_init(&empty[s], 4);
         for (int s = 0; s < kPdItems; s++) mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], 8);
         *abort_flag = 0, *never_set = 0;
         mbar_fence_init();
@@ -159,6 +163,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
                 const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1, key0 = kt * kTile;
+                uint64_t *landed = &full[g % L::kFull];
                 const int32_t block = pages.of(kt * per_tile); // of this lane's copy
                 const bool want = lane < per_tile && key0 + lane * bt < keys, good = want && uint32_t(block) < a.blocks;
                 if (warp == 8 && kt + 1 == it.kt1 && it.kt1 - it.kt0 < it.tiles) { // where the parts are (read after the last tile)
@@ -171,14 +176,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     if (want) // a bad block's keys are marked by its scales
                         cp_async8(&scl[st * L::kPages + lane], good ? a.scales + (size_t(block) * a.kv_heads + it.head) * 2
                                                                     : reinterpret_cast<const float *>(a.words + kPagedBadScale));
-                    cp_async_arrive(&full[st]);
+                    cp_async_arrive(landed);
                     continue;
                 }
                 const uint32_t copies = __popc(__ballot_sync(0xffffffffu, good));
-                if (lane == 0) mbar_expect_tx(&full[st], copies * bt * D);
+                if (lane == 0) mbar_expect_tx(landed, copies * bt * D);
                 __syncwarp();
                 if (good)
-                    tma_load_3d(ring + st * L::kStage + (warp == 9 ? L::kSide : 0) + lane * bt * D, warp == 9 ? &map_v : &map_k, &full[st], 0,
+                    tma_load_3d(ring + st * L::kStage + (warp == 9 ? L::kSide : 0) + lane * bt * D, warp == 9 ? &map_v : &map_k, landed, 0,
                                 int((uint32_t(block) * a.kv_heads + it.head) * a.block_tokens + ((key0 + lane * bt) & (a.block_tokens - 1))), 0);
             }
         }
@@ -188,7 +193,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         // let what was issued land before the shared memory goes
         const uint32_t from = g > L::kStages ? g - L::kStages : 0;
-        for (uint32_t k = from; k < g; k++) mbar_wait(&full[k % L::kStages], (k / L::kStages) & 1, never_set, 200000u);
+        for (uint32_t k = from; k < g; k++) mbar_wait(&full[k % L::kFull], (k / L::kFull) & 1, never_set, 200000u);
         return;
     }
 
@@ -260,8 +265,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int32_t vis = it.vis;
         for (uint32_t kt = it.kt0; kt < it.kt1; kt++, g++) {
             if ((g & 1) != team) continue;
-            const uint32_t st = g % L::kStages, ph = (g / L::kStages) & 1;
-            if (ok && !mbar_wait(&full[st], ph, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
+            const uint32_t st = g % L::kStages;
+            if (ok && !mbar_wait(&full[g % L::kFull], (g / L::kFull) & 1, abort_flag)) { give_up(kStatusFullTimeout); ok = false; }
             if (!ok) continue;
             const int32_t key0 = int32_t(kt * kTile + sub * 16 * U);
             if (key0 < vis) {
