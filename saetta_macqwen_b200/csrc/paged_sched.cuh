@@ -83,9 +83,20 @@ struct PagedShare {
 __device__ __forceinline__ uint32_t paged_ctas(uint64_t total, uint32_t min_tiles) {
     return uint32_t(min(uint64_t(gridDim.x), max(uint64_t(1), total >> 32 ? total / min_tiles : uint64_t((uint32_t(total) + min_tiles - 1) / min_tiles))));
 }
-// total * c / n for a CTA number c <= n < 256: in 32 bits where that holds (a division of 64-bit numbers takes some 500 clocks).
-__device__ __forceinline__ uint64_t paged_cut(uint64_t total, uint32_t c, uint32_t n) {
-    return total < (1u << 24) ? uint32_t(total) * c / n : total * c / n;
+// total * c / n for a CTA number c <= n < 256.  No division of 64-bit numbers: that is a call, and this and what follows run in warps that have given
+// registers back, where a callee compiled for the launch's number may use some that are gone.  In 32 bits where that holds; else 16 bits
+// of the dividend at a time (a remainder and 16 bits stay below 2^24).
+__host__ __device__ __forceinline__ uint64_t paged_cut(uint64_t total, uint32_t c, uint32_t n) {
+    if (total < (1u << 24)) return uint32_t(total) * c / n;
+    const uint64_t x = total * c;
+    uint64_t q = 0;
+    uint32_t rest = 0;
+#pragma unroll 1
+    for (int at = 48; at >= 0; at -= 16) {
+        const uint32_t y = rest << 16 | (uint32_t(x >> at) & 0xffffu);
+        q = q << 16 | y / n, rest = y % n;
+    }
+    return q;
 }
 
 // Walks the items of a share; every role of a CTA walks the same ones.
@@ -130,11 +141,19 @@ struct PagedWalk {
 __device__ __forceinline__ int32_t paged_visible(const PagedItem &it) { return min(int32_t(it.q.kv), it.lim0 + int32_t(it.ntok) - 1); }
 
 // The CTA whose share holds tile x.
-static __device__ __noinline__ uint32_t paged_cta_of(uint64_t total, uint32_t ctas, uint64_t x) {
-    uint32_t c = total < (1u << 24) ? uint32_t(x) * ctas / uint32_t(total) : uint32_t(x * ctas / total);
-    while (paged_cut(total, c + 1, ctas) <= x) c++;
-    while (paged_cut(total, c, ctas) > x) c--;
-    return c;
+__host__ __device__ __forceinline__ uint32_t paged_cta_of(uint64_t total, uint32_t ctas, uint64_t x) {
+    if (total < (1u << 24)) { // the quotient is the CTA or the one after it, whose share would begin behind x
+        const uint32_t c = uint32_t(x) * ctas / uint32_t(total);
+        return c + (c + 1 < ctas && uint32_t(total) * (c + 1) / ctas <= uint32_t(x));
+    }
+    uint32_t lo = 0, hi = ctas;
+#pragma unroll 1
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (paged_cut(total, mid, ctas) <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
 }
 // The CTAs that an item's tiles lie in: the first, and how many.
 __device__ __forceinline__ uint2 paged_ctas_of(const PagedShare &s, const PagedItem &it) {

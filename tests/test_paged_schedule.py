@@ -1,0 +1,53 @@
+"""How a paged attention launch divides its tiles, on the CPU: the schedule's arithmetic, compiled for the host from the kernels' own
+header, against plain integers."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+CSRC = os.path.join(HERE, "..", "saetta_macqwen_b200", "csrc")
+HOST = """
+#include "paged_sched.cuh"
+extern "C" uint64_t cut(uint64_t total, uint32_t c, uint32_t n) { return saetta::paged_cut(total, c, n); }
+extern "C" uint32_t cta_of(uint64_t total, uint32_t ctas, uint64_t x) { return saetta::paged_cta_of(total, ctas, x); }
+"""
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    d = tmp_path_factory.mktemp("sched")
+    (d / "host.cu").write_text(HOST)
+    subprocess.run(["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-I", CSRC, "-shared", "-Xcompiler", "-fPIC", "-o", str(d / "host.so"),
+                    str(d / "host.cu")], check=True, capture_output=True)
+    lib = C.CDLL(str(d / "host.so"))
+    lib.cut.restype = C.c_uint64
+    lib.cut.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32]
+    lib.cta_of.restype = C.c_uint32
+    lib.cta_of.argtypes = [C.c_uint64, C.c_uint32, C.c_uint64]
+    return lib
+
+
+def totals(rng, n):
+    yield from (1, 2, 148, 255, (1 << 24) - 1, 1 << 24, (1 << 32) + 7, (1 << 48) + 12345)
+    for _ in range(n):
+        yield rng.randrange(1, 1 << rng.randint(1, 50))
+
+
+def test_shares_are_equal_and_cover_every_tile(host):
+    rng = random.Random(1)
+    for total in totals(rng, 3000):
+        n = rng.randint(1, 255)
+        for c in {0, n, rng.randint(0, n)}:
+            assert host.cut(total, c, n) == total * c // n
+
+
+def test_the_cta_of_a_tile_is_the_one_whose_share_holds_it(host):
+    rng = random.Random(2)
+    for total in totals(rng, 3000):
+        n = rng.randint(1, min(255, total))
+        for x in {0, total - 1, rng.randrange(total), total // 2}:
+            c = host.cta_of(total, n, x)
+            assert 0 <= c < n and total * c // n <= x < total * (c + 1) // n
