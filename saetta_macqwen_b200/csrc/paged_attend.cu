@@ -124,7 +124,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     if (tid == kPdThreads - 1) prefetch_map(&map_k), prefetch_map(&map_v);
     pdl_wait();
-    paged_share<kTile>(a, tpt, kPdThreads, 1, scratch, share);
+    paged_share<kTile>(a, tpt, kPdThreads, scratch, share);
     if (share->x0 >= share->x1) return;
     auto give_up = [&](uint32_t bit) {
         atomicOr(a.words, bit);

@@ -268,7 +268,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         mbar_fence_init();
     }
     pdl_wait();
-    paged_share<kPpKeys>(a, tpt, kPpThreads, 1, reinterpret_cast<uint64_t *>(sQ), share); // (its scratch is the Q area, free until the roles begin)
+    paged_share<kPpKeys>(a, tpt, kPpThreads, reinterpret_cast<uint64_t *>(sQ), share); // (its scratch is the Q area, free until the roles begin)
     if (share->x0 >= share->x1) return; // (the whole CTA)
     if (warp == 21) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");

@@ -8,21 +8,18 @@
 
 namespace saetta {
 
-// (Called, not copied into every caller, as is what divides 64-bit numbers below: the kernels' code has to stay well below the 128 KB
-// that an SM keeps of it; past that every instruction is fetched from far away.)
-// sum over i < n of floor((a i + b) / m): counts lattice points under the line, exchanging slope and modulus as Euclid's
-// algorithm does.
-static __device__ __noinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
-    uint64_t sum = 0;
-    while (true) {
-        if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
-        if (b >= m) sum += n * (b / m), b %= m;
-        const uint64_t top = a * n + b;
-        if (top < m) return sum;
-        n = top / m, b = top % m;
-        const uint64_t t = m;
-        m = a, a = t;
-    }
+// sum over i < n of floor((a i + b) / T), T a power of two, a > 0: the numerators' sum less that of their remainders, by T.  With g the largest power
+// of two that divides a (T at most), the remainders of T / g numerators in a row are, in some order, b mod g and every step of g above it up
+// to T: whole periods cost nothing, and fewer than T / g terms are left to be added one by one.
+template <uint32_t T>
+__host__ __device__ __forceinline__ uint64_t tile_sum(uint32_t n, uint32_t a, uint64_t b) {
+    static_assert((T & (T - 1)) == 0 && T > 1, "a power of two");
+    const uint32_t low = a & (0u - a), g = low < T ? low : T, period = T / g, left = n & (period - 1);
+    uint64_t rest = uint64_t(n / period) * (period * (uint32_t(b) & (g - 1)) + T / 2 * (period - 1));
+    uint32_t x = uint32_t(b);
+#pragma unroll 1
+    for (uint32_t i = 0; i < left; i++, x += a) rest += x & (T - 1);
+    return (uint64_t(n) * (n - 1) / 2 * a + uint64_t(n) * b - rest) / T;
 }
 
 // A sequence as the kernels read it: its rows [row0, row0 + n) of q, its keys [0, kv).
@@ -49,11 +46,11 @@ struct PagedTiles {
     }
     // at least one tile, so that rows that see no key are written too
     __device__ __forceinline__ uint32_t count(const PagedSeq &q, uint32_t r) const { return max(1u, (keys(q, r) + T - 1) / T); }
-    __device__ __noinline__ uint64_t before(const PagedSeq &q, uint32_t r) const { // of row tiles 0 .. r - 1
+    __device__ __forceinline__ uint64_t before(const PagedSeq &q, uint32_t r) const { // of row tiles 0 .. r - 1
         if (!r) return 0;
         if (q.kv < q.n) return uint64_t(r) * count(q, 0);
         const uint32_t full = r == row_tiles(q) ? r - 1 : r;
-        uint64_t sum = full ? floor_sum(full, T, tpt, q.kv - q.n + tpt + T - 1) : 0;
+        uint64_t sum = full ? tile_sum<T>(full, tpt, q.kv - q.n + tpt + T - 1) : 0;
         if (full != r) sum += count(q, r - 1);
         return sum;
     }
@@ -79,10 +76,8 @@ struct PagedShare {
     PagedSeq q;             // of `seq`
 };
 
-// The CTAs that get a share: none of them less than min_tiles.
-__device__ __forceinline__ uint32_t paged_ctas(uint64_t total, uint32_t min_tiles) {
-    return uint32_t(min(uint64_t(gridDim.x), max(uint64_t(1), total >> 32 ? total / min_tiles : uint64_t((uint32_t(total) + min_tiles - 1) / min_tiles))));
-}
+// The CTAs that get a share.
+__device__ __forceinline__ uint32_t paged_ctas(uint64_t total) { return uint32_t(min(uint64_t(gridDim.x), max(uint64_t(1), total))); }
 // total * c / n for a CTA number c <= n < 256.  No division of 64-bit numbers: that is a call, and this and what follows run in warps that have given
 // registers back, where a callee compiled for the launch's number may use some that are gone.  In 32 bits where that holds; else 16 bits
 // of the dividend at a time (a remainder and 16 bits stay below 2^24).
@@ -164,7 +159,7 @@ __device__ __forceinline__ uint2 paged_ctas_of(const PagedShare &s, const PagedI
 
 // Finds this CTA's share.  All `threads` threads of the block call it; `scratch` (40 words of 8 bytes) and `share` are shared memory.
 template <int T>
-__device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, uint32_t threads, uint32_t min_tiles, uint64_t *scratch, PagedShare *share) {
+__device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, uint32_t threads, uint64_t *scratch, PagedShare *share) {
     const PagedTiles<T> tiles{tpt};
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
     uint64_t total = 0, x0 = 0;
@@ -206,14 +201,14 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
             v += before; // inclusive
             if (once || pass == 0) total = carry + all;
             if (once) {
-                const uint32_t ctas = paged_ctas(total, min_tiles);
+                const uint32_t ctas = paged_ctas(total);
                 x0 = blockIdx.x < ctas ? paged_cut(total, blockIdx.x, ctas) : total;
             }
             if (pass == 1 && cost && v - cost <= x0 && x0 < v) share->seq = s, share->head_base = v - cost, share->q = q, share->per_head = per;
             carry += all;
             __syncthreads();
         }
-        const uint32_t ctas = paged_ctas(total, min_tiles);
+        const uint32_t ctas = paged_ctas(total);
         x0 = blockIdx.x < ctas ? paged_cut(total, blockIdx.x, ctas) : total;
         if (tid == 0) {
             share->total = total, share->ctas = ctas, share->x0 = x0;

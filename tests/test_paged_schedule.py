@@ -13,6 +13,8 @@ HOST = """
 #include "paged_sched.cuh"
 extern "C" uint64_t cut(uint64_t total, uint32_t c, uint32_t n) { return saetta::paged_cut(total, c, n); }
 extern "C" uint32_t cta_of(uint64_t total, uint32_t ctas, uint64_t x) { return saetta::paged_cta_of(total, ctas, x); }
+extern "C" uint64_t sum64(uint32_t n, uint32_t a, uint64_t b) { return saetta::tile_sum<64>(n, a, b); }
+extern "C" uint64_t sum128(uint32_t n, uint32_t a, uint64_t b) { return saetta::tile_sum<128>(n, a, b); }
 """
 
 
@@ -27,6 +29,9 @@ def host(tmp_path_factory):
     lib.cut.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32]
     lib.cta_of.restype = C.c_uint32
     lib.cta_of.argtypes = [C.c_uint64, C.c_uint32, C.c_uint64]
+    for f in (lib.sum64, lib.sum128):
+        f.restype = C.c_uint64
+        f.argtypes = [C.c_uint32, C.c_uint32, C.c_uint64]
     return lib
 
 
@@ -51,3 +56,19 @@ def test_the_cta_of_a_tile_is_the_one_whose_share_holds_it(host):
         for x in {0, total - 1, rng.randrange(total), total // 2}:
             c = host.cta_of(total, n, x)
             assert 0 <= c < n and total * c // n <= x < total * (c + 1) // n
+
+
+@pytest.mark.parametrize("tpt", sorted({max(1, r // g) for r in (8, 16, 128) for g in range(1, 17)}))
+def test_the_tiles_of_row_tiles(host, tpt):
+    """Key tiles of the first n row tiles of tpt tokens, the first of which sees b - T + 1 keys."""
+    rng = random.Random(tpt)
+    for f, T in ((host.sum64, 64), (host.sum128, 128)):
+        for n in (0, 1, 2, 7, 127, 128, 129, rng.randrange(1000), rng.randrange(1 << 16)):
+            for b in (0, 1, T - 1, T, rng.randrange(1 << 20), rng.randrange(1 << 31)):
+                assert f(n, tpt, b) == sum((tpt * i + b) // T for i in range(n))
+
+
+def test_nothing_is_called_after_registers_were_given_back():
+    """A callee compiled for the launch's registers may use some that its warp no longer has: these kernels call nothing at all."""
+    for name in ("paged_sched.cuh", "paged_attend.cu", "paged_prefill.cu"):
+        assert "__noinline__" not in open(os.path.join(CSRC, name)).read(), name
