@@ -514,7 +514,7 @@ int saetta_paged_attention_create(int device, size_t heads, size_t kv_heads, siz
     auto *op = new (std::nothrow) saetta_paged_attention();
     if (!op) return fail(SAETTA_ERR_NO_MEM, "PagedAttention: host allocation");
     op->device = device, op->heads = heads, op->kv_heads = kv_heads, op->head_dim = head_dim;
-    op->ctas = std::min(sm_count(device), 255); // (paged_cut)
+    op->ctas = std::min(sm_count(device), kPagedMaxCtas);
     op->part_floats = 128 * (head_dim + 2) + 4; // 128 rows: the largest tile; (m, l) of each; the value scale O is kept by
     void *p = nullptr, *w = nullptr;
     const size_t words = size_t(kPagedCounters) + 3 * size_t(op->ctas);

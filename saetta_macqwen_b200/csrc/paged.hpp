@@ -29,6 +29,9 @@ constexpr int kPagedBadScale = 2;         // word index of the (-1, -1) pair
 constexpr int kPagedCounters = 8;
 constexpr int kPagedMaxGroup = 16;        // query heads of one kv head
 constexpr size_t kPagedMaxSeqs = 8192;
+// CTAs of an attention launch, at most.  Parts of an item are joined in two rounds of groups of ceil(sqrt(parts)): 13 is what the few-rows
+// kernel has registers for.  (paged_cut's 32-bit steps hold up to 255.)
+constexpr int kPagedMaxCtas = 13 * 13;
 // Rows (tokens x heads of a kv head) of a sequence up to which the few-rows kernel runs: what two products' columns hold.  Measured, few-rows against
 // many-rows kernel: 24 sequences of 4700 keys, heads of 256, 8 rows 39 us and 63, 16 rows 71 and 67; heads of 128, 8 rows 63 and 110, 16 rows 75 and
 // 117; one sequence of 700 keys, 16 rows 21 and 35; 24 sequences of some 3000 keys, 32 rows 138 (in two passes over the keys) and 96.

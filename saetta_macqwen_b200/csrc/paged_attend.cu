@@ -31,7 +31,8 @@
 namespace saetta {
 
 constexpr int kPdThreads = 384;  // 8 consumer warps; items and keys, values, scales; one warp that makes up the group of 4
-constexpr uint32_t kPdGroup = 12; // parts of an item that one CTA joins by itself
+constexpr uint32_t kPdGroup = 12; // parts of an item that one CTA joins by itself; one more in each of two rounds
+static_assert((kPdGroup + 1) * (kPdGroup + 1) >= uint32_t(kPagedMaxCtas), "two rounds join the parts of every CTA");
 constexpr float kPdRescale = 8.f; // the accumulators follow the running maximum only past this many doublings
 
 template <int D, int NT>

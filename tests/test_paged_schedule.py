@@ -3,6 +3,7 @@ header, against plain integers."""
 import ctypes as C
 import os
 import random
+import re
 import subprocess
 
 import pytest
@@ -72,3 +73,17 @@ def test_nothing_is_called_after_registers_were_given_back():
     """A callee compiled for the launch's registers may use some that its warp no longer has: these kernels call nothing at all."""
     for name in ("paged_sched.cuh", "paged_attend.cu", "paged_prefill.cu"):
         assert "__noinline__" not in open(os.path.join(CSRC, name)).read(), name
+
+
+def test_two_rounds_join_the_parts_of_every_cta():
+    """A round of the few-rows kernel holds kPdGroup + 1 parts at once, for as many CTAs as a launch may have."""
+    hpp, attend = (open(os.path.join(CSRC, n)).read() for n in ("paged.hpp", "paged_attend.cu"))
+    a, b = map(int, re.search(r"kPagedMaxCtas = (\d+) \* (\d+);", hpp).groups())
+    group = int(re.search(r"kPdGroup = (\d+);", attend).group(1))
+    for parts in range(1, a * b + 1):
+        per = parts
+        if parts > group:
+            per = 2
+            while per * per < parts:
+                per += 1
+        assert per <= group + 1 and (parts + per - 1) // per <= group + 1, parts
