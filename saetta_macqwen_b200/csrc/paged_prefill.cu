@@ -791,6 +791,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     if (warp == 0 && lane == 0) part_of(0)[kPpRows * (D + 2)] = vtop; // (row 0 is always live)
                     lo = 0, step = per, n = groups, counter = a.words + kPagedCounters + 2 * gridDim.x + c0;
                 }
+                PP_MEET_ALL(); // the joined sums have been read: the next item's maxima may take their place
             }
         }
     }
