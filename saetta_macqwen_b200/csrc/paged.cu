@@ -307,6 +307,8 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
             __syncthreads(); // (and `was` has been read)
 #pragma unroll
             for (int w = 0; w < 8; w++) amax = fmaxf(amax, red[w]);
+        } else {
+            __syncwarp(); // `was` has been read by every lane
         }
         uint8_t *page = (side ? a.values : a.keys) + (size_t(block) * a.kv_heads + head) * B * D;
         const float fresh = pow2_scale(amax), scale = off ? fmaxf(fresh, was) : fresh;

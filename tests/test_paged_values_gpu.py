@@ -24,3 +24,22 @@ def test_a_cta_that_joins_an_item_and_goes_on_to_another():
         torch.cuda.synchronize()
         assert torch.equal(first, c.out)
     assert op.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", [sa.F32, sa.BF16])
+def test_short_runs_that_raise_a_scale_read_it_before_it_is_written(dt):
+    """One lane writes a block's scale that all lanes of the warp have read: single rows of as many sequences, each larger than what its
+    block holds."""
+    import torch
+
+    from paged_util import ref_store
+    from test_paged_gpu import Pool, i32, tdt
+
+    p = Pool(2, 256, 64, 300, seed=3)
+    rng = np.random.default_rng(3)
+    slots = [b * 64 + int(rng.integers(1, 64)) for b in range(300)]
+    k, v = (torch.from_numpy((rng.normal(size=(300, 2, 256)) * 2.0 ** rng.integers(-3, 9, (300, 1, 1))).astype(np.float32)).to(tdt(dt)) for _ in range(2))
+    p.cache.store(k.cuda(), v.cuda(), i32(slots), 300, dtype=dt)
+    torch.cuda.synchronize()
+    ref_store(*p.codes, p.scales, k.double().numpy(), v.double().numpy(), slots, 64)
+    p.same()
