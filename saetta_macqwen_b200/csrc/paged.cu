@@ -467,7 +467,8 @@ int saetta_paged_assign(int device, size_t seqs, size_t block_tokens, const uint
                        slots_dev, positions_dev, kv_lens_out_dev, free_count_out_dev, status_dev, uint32_t(seqs), uint32_t(table_stride),
                        uint32_t(shift), uint32_t(free_cap), uint32_t(rows_cap)};
     const size_t smem = 4 * (seqs + 1) * sizeof(uint32_t);
-    if (smem > 48 * 1024) SAETTA_CUDA(cudaFuncSetAttribute(paged_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(4 * (kPagedMaxSeqs + 1) * 4)));
+    // 48 KB hold what a launch has without asking, the kernel's static shared memory (some 400 bytes) included
+    if (smem > 47 * 1024) SAETTA_CUDA(cudaFuncSetAttribute(paged_assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(4 * (kPagedMaxSeqs + 1) * 4)));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     const unsigned ctas = rows_cap > 4096 ? 8 : 1;

@@ -43,3 +43,28 @@ def test_short_runs_that_raise_a_scale_read_it_before_it_is_written(dt):
     torch.cuda.synchronize()
     ref_store(*p.codes, p.scales, k.double().numpy(), v.double().numpy(), slots, 64)
     p.same()
+
+
+FRESH = """
+import sys
+sys.path[:0] = {path!r}
+import torch
+from test_paged_gpu import Step
+for seqs in (3046, 3047, 3071, 3072, 8192):
+    st = Step([5] * seqs, [1] * seqs, None, [0] * 4, 4, [[0]] * seqs, 16, seqs)
+    st.run()
+    torch.cuda.synchronize()
+    assert st.status.item() == 0 and st.starts[-1].item() == seqs and st.slots.cpu().tolist() == [5] * seqs, seqs
+print("done")
+"""
+
+
+def test_assign_of_every_number_of_sequences_in_a_process_that_made_no_larger_call():
+    """Its scan's shared memory passes what a launch has without asking at 3047 sequences."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FRESH.format(path=[here, os.path.dirname(here)])], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
