@@ -71,7 +71,7 @@ struct PpLayout {
     static constexpr int kRing = (kKStages + kVStages) * kStage;
     // the statistics' area: maxima, scales, items, the share, barriers, four words, the rows' exponents
     static constexpr int kBarriers = 2 * (kKStages + kVStages) + 2 * kPpScaleRing + 2 * kPpItems + 3 * 2 + 6 + 16;
-    static constexpr int kStats = 4 * 2 * kPpRows * 2 + kPpScaleRing * kPpScales * 8 + kPpItems * int(sizeof(PpItem)) + int(sizeof(PagedShare)) + kBarriers * 8 + 16 + kPpRows;
+    static constexpr int kStats = 4 * kPpRows * 4 + kPpScaleRing * kPpScales * 8 + kPpItems * int(sizeof(PpItem)) + int(sizeof(PagedShare)) + kBarriers * 8 + 16 + kPpRows;
     static_assert((kPpItems * sizeof(PpItem)) % 8 == 0 && sizeof(PagedShare) % 8 == 0, "barriers stand at multiples of 8 bytes");
     static constexpr int kSmem = PARTS * kQPart + kRing + kStats;
     // O; the scores of one tile; the weights' buffers, one or two
@@ -218,6 +218,12 @@ __device__ __forceinline__ bool short_wait(uint64_t *bar, uint32_t parity) {
         : "memory");
     return __all_sync(0xffffffffu, ok != 0);
 }
+// An f32 value as an unsigned integer, of the same order (0 is below them all), for the largest of several by atomicMax; and back.
+__device__ __forceinline__ uint32_t in_order(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float(u ^ (uint32_t(int32_t(~u) >> 31) | 0x80000000u)); }
 __device__ __forceinline__ float lg2_approx(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -234,10 +240,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     uint8_t *ring = sQ + PARTS * L::kQPart;              // [K stages, V stages][slab][128 keys][128 dims]
     uint8_t *ring_v = ring + NK * L::kStage;
     // the statistics' area
-    __nv_bfloat16 *xch = reinterpret_cast<__nv_bfloat16 *>(ring + L::kRing); // [4 tiles][2 halves][128 rows]: maxima, rounded up
-    float *lx = reinterpret_cast<float *>(xch);                              // at a tile's end: [4][128 rows] sums
-    float2 *scl = reinterpret_cast<float2 *>(xch + 1024);                    // [kPpScaleRing][8]: key scale (-1: bad block), log2 r; then
-                                                                             // what vref falls by against the tile before
+    uint32_t *xch = reinterpret_cast<uint32_t *>(ring + L::kRing); // [4 tiles][128 rows]: maxima, as in_order gives them; 0: none yet
+    float *lx = reinterpret_cast<float *>(xch);                    // at a tile's end: [4][128 rows] sums
+    float2 *scl = reinterpret_cast<float2 *>(xch + 4 * kPpRows);   // [kPpScaleRing][8]: key scale (-1: bad block), log2 r; then
+                                                                   // what vref falls by against the tile before
     PpItem *items = reinterpret_cast<PpItem *>(scl + kPpScaleRing * kPpScales);
     PagedShare *share = reinterpret_cast<PagedShare *>(items + kPpItems);
     uint64_t *bars = reinterpret_cast<uint64_t *>(share + 1);
@@ -255,6 +261,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         if (threadIdx.x == 0) atomicOr(a.words, kStatusMmaTimeout);
         return;
     }
+    if (threadIdx.x < 4 * kPpRows) xch[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NK; s++) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
         for (int s = 0; s < NV; s++) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
@@ -539,7 +546,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             // The running maximum after a tile whose own is `top` (the same in all four warps that share the rows).
             auto follow = [&](float was, float top) {
                 const bool need = __any_sync(0xffffffffu, top > was + kPpRescale<PARTS>);
-                return need ? fmaxf(was, __bfloat162float(__float2bfloat16_ru(top + kPpSpare))) : was;
+                return need ? fmaxf(was, top + kPpSpare) : was;
             };
             for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
                 if ((g & 1) != team) continue;
@@ -572,22 +579,23 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     t[0] = max3(t[0], x[6], x[7]), t[1] = max3(t[1], x[8], x[9]), t[0] = max3(t[0], x[10], x[11]), t[1] = max3(t[1], x[12], x[13]);
                     mx = fmaxf(mx, fmaxf(max3(t[0], x[14], x[15]), t[1]) * fmaxf(fabsf(f) * rs, FLT_MIN)); // (not 0: that times a masked key's -infinity is NaN)
                 }
-                // The two threads of a row agree on one maximum (rounded up it is still one that no score passes).  Every warp follows the running
-                // maximum through all tiles: the other team's tile first, then its own.  (Waiting for the other team's tile also shows
-                // that its slot of four tiles ago has been read.)
+                // The two threads of a row agree on one maximum.  Every warp follows the running maximum through all tiles: the other team's tile first,
+                // then its own.  (The maxima go through shared memory in f32: in bfloat16, whatever way it is rounded, one of 1000 is off by
+                // several doublings, and the weights with it.)  A slot is cleared three tiles after its own, by the other team: waiting for the
+                // tile before this one has shown that all four warps of these rows are past the two tiles in which they read it.
                 const uint32_t xs = g & 3;
                 float m_was = -INFINITY;
                 if (kt > kt0) {
                     const uint32_t xo = (g - 1) & 3;
                     PP_WAIT(&x_met[xo * 4 + quarter], (g - 1) >> 2 & 1);
-                    m_was = follow(m, fmaxf(__bfloat162float(xch[xo * 256 + row]), __bfloat162float(xch[xo * 256 + 128 + row])));
+                    m_was = follow(m, from_order(xch[xo * kPpRows + row]));
                 }
-                const __nv_bfloat16 up = __float2bfloat16_ru(mx);
-                xch[xs * 256 + half * 128 + row] = up;
+                if (half == 0) xch[((g + 1) & 3) * kPpRows + row] = 0;
+                atomicMax(&xch[xs * kPpRows + row], in_order(mx));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&x_met[xs * 4 + quarter]);
                 PP_WAIT(&x_met[xs * 4 + quarter], g >> 2 & 1);
-                const float mt = follow(m_was, fmaxf(__bfloat162float(up), __bfloat162float(xch[xs * 256 + (half ^ 1) * 128 + row])));
+                const float mt = follow(m_was, from_order(xch[xs * kPpRows + row]));
                 if (mt != m) {
                     l *= ex2_approx(m - mt); // 0 for the first
                     m = mt;
@@ -663,7 +671,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     PP_WAIT(all_met, all++ & 1)
             if (((g - 1) & 1) != team) { // the last tile was the other team's
                 PP_WAIT(&x_met[((g - 1) & 3) * 4 + quarter], (g - 1) >> 2 & 1);
-                const float mt = follow(m, fmaxf(__bfloat162float(xch[((g - 1) & 3) * 256 + row]), __bfloat162float(xch[((g - 1) & 3) * 256 + 128 + row])));
+                const float mt = follow(m, from_order(xch[((g - 1) & 3) * kPpRows + row]));
                 if (mt != m) l *= ex2_approx(m - mt);
                 m = mt;
             }
@@ -791,8 +799,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     if (warp == 0 && lane == 0) part_of(0)[kPpRows * (D + 2)] = vtop; // (row 0 is always live)
                     lo = 0, step = per, n = groups, counter = a.words + kPagedCounters + 2 * gridDim.x + c0;
                 }
-                PP_MEET_ALL(); // the joined sums have been read: the next item's maxima may take their place
+                PP_MEET_ALL(); // the joined sums have been read
             }
+            xch[threadIdx.x] = 0; // the next item's maxima take the sums' place
+            PP_MEET_ALL();
         }
     }
     goto done;

@@ -1,0 +1,51 @@
+"""Attention over the paged cache on the GPU, for keys, values and scores that models have and random ones do not."""
+import numpy as np
+import pytest
+
+import saetta_macqwen_b200 as sa
+from paged_values import Sequences, bf16
+
+pytestmark = pytest.mark.gpu
+
+# The yardstick: the same softmax in 64 bits with its weights rounded to bfloat16, as an ordinary kernel has them.  The kernels may be
+# off by twice that as a whole, and by what f32 scores make of the weights: a score is a running sum of some 2 * dim / 32 steps (three terms: 3),
+# each off by at most 2^-22 of the largest partial sum, which the tests keep near the score itself.
+
+HEADS, DIM = 8, 128
+
+
+def parts(q_dt):
+    return 2 if q_dt == sa.BF16 else 3
+
+
+def allowed(s, want, absv, top):
+    coarse, _, _ = s.exact(bf16)
+    return 2 * np.linalg.norm(coarse - want) + np.linalg.norm(absv * (parts(s.q_dt) * s.dim / 32 * 2.0 ** -22 * (top[..., None] + 1)))
+
+
+def near(s, got):
+    want, absv, top = s.exact()
+    lim = allowed(s, want, absv, top)
+    assert np.linalg.norm(got - want) <= lim, (np.linalg.norm(got - want) / np.linalg.norm(want), lim / np.linalg.norm(want))
+
+
+def plain(rng, n, kv, dim=DIM, heads=HEADS, mean=1.0):
+    """Scores of one nat's spread once scaled by dim ** -0.5; dim 0 of q is 1 and of k is 0: for offsets."""
+    q, k, v = rng.normal(size=(n, heads, dim)), rng.normal(size=(kv, 1, dim)), rng.normal(size=(kv, 1, dim)) + mean
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    return q, k, v
+
+
+ROWS = [(2, "few"), (24, "many")]  # rows of a sequence: 16 and 192 rows of a tile
+
+
+@pytest.mark.parametrize("rows,kernel", ROWS)
+@pytest.mark.parametrize("q_dt", [sa.BF16, sa.F16])
+@pytest.mark.parametrize("nats", [400, 700, 1500, -700, -1500, 6000])
+def test_an_offset_of_all_scores_changes_nothing(rows, kernel, q_dt, nats):
+    rng = np.random.default_rng(5)
+    q, k, v = plain(rng, rows, 1500)
+    q[..., 0] = nats / 16
+    k[..., 0] = 16 * DIM ** 0.5
+    s = Sequences([(q, k, v)], 64, q_dt, DIM ** -0.5)
+    near(s, s.run())
