@@ -1,6 +1,6 @@
 // Attention of many rows (prompts) over the paged e4m3 cache, on the 5th-generation tensor cores.
 //
-//   s_ij = scale (q_i . kcode_j) ks[block(j)] log2 e,   r_j = vs[block(j)] / vref,   w = 2^(s - max s + log2 r)
+//   s_ij = scale (q_i . kcode_j) ks[block(j)] log2 e,   r_j = vs[block(j)] / vref,   w = 2^(s + log2 r - m),  m some max(s + log2 r)
 //   out_i = vref sum_j w_ij vcode_j / sum_j (w_ij / r_j)
 //
 // The codes are the operands as they lie in memory: no conversion of K or V.  tcgen05's 8-bit products run at twice the
@@ -8,8 +8,8 @@
 // significant bits (bfloat16 q) is the sum of two (4 bits each), one of 11 (binary16 q) of three.  Two products at the 8-bit rate take
 // the time of one at the 16-bit rate, with half the shared memory for K and V.  The value scales go into the exponent,
 // relative to the largest so far (vref, by which O is kept), so a block's scales cost nothing for each score but the constants of one FMA, and
-// the sum of the softmax takes them out again for each 16 keys.  (r is not let below 2^-40: a block of zeros, whose scale is
-// 2^-126, still counts in the sum; what the bound adds to values is below 2^-40 of the largest.)
+// the sum of the softmax takes them out again for each 16 keys.  (r is not let below 2^-60: a block of zeros, whose scale is
+// 2^-126, still counts in the sum; what the bound adds to values is below 2^-60 of the largest.)
 //
 // A tile is 128 rows: `tpt` tokens x the query heads of one kv head.  Key tiles are 128 keys.  Bound by the tensor pipe: 2 * PARTS *
 // 128 * 128 * D multiply-adds for each tile at 8192 a clock and SM.  Roles: sixteen softmax warps in two teams that take
@@ -43,7 +43,7 @@ template <int PARTS>
 constexpr float kPpShift = PARTS == 3 ? 8.f : 6.f;
 template <int PARTS>
 constexpr float kPpRescale = PARTS == 3 ? 0.5f : 2.5f;
-constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 0.5f;
+constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 0.5f, kPpFall = 11.f, kPpReach = 40.f;
 constexpr uint32_t kPpGroup = 8;  // parts of an item that one CTA joins by itself
 constexpr int kPpScaleRing = 4, kPpScales = 9;
 
@@ -413,7 +413,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
                     for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                     top = fmaxf(fmaxf(__shfl_sync(0xffffffffu, top, 0), FLT_MIN), vref);
-                    v.y = good ? fmaxf(lg2_approx(v.y / top), -40.f) : 0.f;
+                    v.y = good ? fmaxf(lg2_approx(v.y / top), -60.f) : 0.f;
                     if (lane == 8) v = make_float2(vref > 0.f ? vref / top : 1.f, top);
                     vref = top;
                     PP_WAIT(&sc_empty[ss], (g / kPpScaleRing & 1) ^ 1);
@@ -542,11 +542,17 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const float rs = __uint_as_float(uint32_t(row_e[row]) << 23) * a.scale_log2;
             __syncwarp();
             if (lane == 0) mbar_arrive(q_empty); // the factor has been read
-            float m = -INFINITY, l = 0.f;
-            // The running maximum after a tile whose own is `top` (the same in all four warps that share the rows).
+            float m = -INFINITY, l = 0.f, hi = -INFINITY;
+            // What a tile's weights stand against, after a tile whose largest is 2^top (the same in all four warps that share the rows).  `top` is of
+            // s + log2 r over the keys that the row sees: of what they put into O, so that a block of large values which the row hardly or not
+            // yet sees takes no bits from the others.  It goes down as well, so that neither does a key of much weight in an earlier tile, but for
+            // no more than 2^kPpReach below the largest so far: l, the sum without r, stays below 2^(kPpReach + 60 + 31).
             auto follow = [&](float was, float top) {
-                const bool need = __any_sync(0xffffffffu, top > was + kPpRescale<PARTS>);
-                return need ? fmaxf(was, top + kPpSpare) : was;
+                hi = fmaxf(hi, top);
+                const float low = fmaxf(top + kPpSpare, hi - kPpReach);
+                const bool down = low < was - kPpFall && top > -INFINITY;
+                if (!__any_sync(0xffffffffu, top > was + kPpRescale<PARTS> || down)) return was;
+                return down ? low : fmaxf(was, top + kPpSpare);
             };
             for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
                 if ((g & 1) != team) continue;
@@ -577,7 +583,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     const float *x = reinterpret_cast<const float *>(&s[b >> 1][(b & 1) * 16]);
                     float t[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
                     t[0] = max3(t[0], x[6], x[7]), t[1] = max3(t[1], x[8], x[9]), t[0] = max3(t[0], x[10], x[11]), t[1] = max3(t[1], x[12], x[13]);
-                    mx = fmaxf(mx, fmaxf(max3(t[0], x[14], x[15]), t[1]) * fmaxf(fabsf(f) * rs, FLT_MIN)); // (not 0: that times a masked key's -infinity is NaN)
+                    mx = fmaxf(mx, fmaf(fmaxf(max3(t[0], x[14], x[15]), t[1]), fmaxf(fabsf(f) * rs, FLT_MIN), sc[b].y)); // (not 0: that times a masked key's -infinity is NaN)
                 }
                 // The two threads of a row agree on one maximum.  Every warp follows the running maximum through all tiles: the other team's tile first,
                 // then its own.  (The maxima go through shared memory in f32: in bfloat16, whatever way it is rounded, one of 1000 is off by

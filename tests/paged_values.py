@@ -43,6 +43,7 @@ class Sequences:
                 for j in range(need[s]):
                     part = x[j * block:(j + 1) * block]
                     side[tables[s, j], :, :len(part)] = part.transpose(1, 0, 2)
+        self.tables = tables
         self.scales = np.ones((pool, self.kv_heads, 2))
         self.codes = []
         for i, side in enumerate(sides):
@@ -74,9 +75,10 @@ class Sequences:
         assert op.device_status() == 0
         return out.double().cpu().numpy()
 
-    def exact(self, weights=lambda p: p, of=abs):
-        """softmax(scale q k) v; with the weights (the largest of a row is 1) rounded by `weights`.  Also the weighted average of |v|, and the largest |score|."""
-        out, absv = np.zeros((2, self.starts[-1], self.heads, self.dim))
+    def exact(self, weights=lambda p: p):
+        """softmax(scale q k) v; with the weights (the largest of a row is 1) rounded by `weights`.  Also the weighted average of |v|, the largest |score|,
+        and `edge`: over tiles of 128 keys, the largest weight times value scale that the row sees there, times the sum of |code|."""
+        out, absv, edge = np.zeros((3, self.starts[-1], self.heads, self.dim))
         top = np.zeros((self.starts[-1], self.heads))
         G = self.heads // self.kv_heads
         for s, q in enumerate(self.q):
@@ -84,6 +86,8 @@ class Sequences:
             rows = slice(self.starts[s], self.starts[s + 1])
             for h in range(self.heads):
                 k, v = self.kv[0][s][h // G], self.kv[1][s][h // G]
+                vs = np.repeat(self.scales[self.tables[s, :-(-kv // self.block)], h // G, 1], self.block)[:kv]
+                code = np.abs(v / vs[:, None])
                 for i0 in range(0, n, 64):
                     i1 = min(n, i0 + 64)
                     w = q[i0:i1, h] @ k.T * self.scale
@@ -96,7 +100,10 @@ class Sequences:
                     out[at] = weights(p) @ v / np.where(t > 0, t, 1)
                     absv[at] = p @ np.abs(v) / np.where(t > 0, t, 1)
                     top[at] = np.where(seen, np.abs(w), 0).max(1)
-        return out, absv, top
+                    for j in range(0, kv, 128):
+                        t128 = slice(j, j + 128)
+                        edge[at] += (p[:, t128] * vs[t128]).max(1, keepdims=True) * (seen[:, t128] @ code[t128]) / np.where(t > 0, t, 1)
+        return out, absv, top, edge
 
 
 def off(a, b):
