@@ -5,7 +5,7 @@
 //
 // The codes are the operands as they lie in memory: no conversion of K or V.  tcgen05's 8-bit products run at twice the
 // 16-bit rate, and the two left-hand operands, which are not 8-bit, are split into sums of e4m3 values: a value of 8
-// significant bits (bfloat16 q) is the sum of two (4 bits each), one of 11 (binary16 q) of three.  Two products at the 8-bit rate take
+// significant bits (bfloat16 q) is the sum of two (4 bits each), one of 11 (binary16 q) of three; of a weight's terms all but the first are e5m2.  Two products at the 8-bit rate take
 // the time of one at the 16-bit rate, with half the shared memory for K and V.  The value scales go into the exponent,
 // relative to the largest so far (vref, by which O is kept), so a block's scales cost nothing for each score but the constants of one FMA, and
 // the sum of the softmax takes them out again for each 16 keys.  (r is not let below 2^-60: a block of zeros, whose scale is
@@ -33,17 +33,13 @@ namespace saetta {
 constexpr int kPpRows = 128, kPpKeys = 128, kPpThreads = 768;
 constexpr int kPpWarps = 16;  // of the softmax: two teams of eight, which take the tiles by turns
 constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the values
-// e4m3 ends at 448 = 2^8.8, and its smallest steps should lie low beside the weights: w is kept times 2^6, by a maximum that O follows only when a
-// row's scores pass it by 2.5 doublings (w stays below 2^8.5); then all 32 rows of the warp are brought up to date, with half a doubling to
-// spare.  (With each row following for itself past 2 doublings, some row of a CTA did so in every other tile of a random prompt of 8192 keys,
-// and the products wait for it; now in one of ten.)  With three terms the smallest steps, and not the last term's rounding, are what
-// remains: w is kept times 2^8 and the maximum follows past half a doubling.  (Over 7 prompts of up to 3500 keys, against 64 bits: 2^5.5 and 3
-// doublings 0.00046 in 634 us, 2^8 and a half 0.00030 in 653 us; a binary16 output alone is off by 0.00021.)
-template <int PARTS>
-constexpr float kPpShift = PARTS == 3 ? 8.f : 6.f;
-template <int PARTS>
-constexpr float kPpRescale = PARTS == 3 ? 0.5f : 2.5f;
-constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 0.5f, kPpFall = 11.f, kPpReach = 40.f;
+// A weight's first term is e4m3, which ends at 448 = 2^8.8: w is kept times 2^6, against a maximum that O follows only when a row's scores pass it by
+// 2.5 doublings (w stays below 2^8.5); then all 32 rows of the warp are brought up to date, with one doubling to spare: a
+// whole one, so that the weight it stands by is a power of two and not rounded (a key of nearly all weight, or a row's only one).  (With each row
+// following for itself past 2 doublings, some row of a CTA did so in every other tile of a random prompt of 8192 keys, and the products wait for
+// it; now in one of ten.)
+constexpr float kPpShift = 6.f, kPpRescale = 2.5f;
+constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 1.f, kPpFall = 8.f, kPpReach = 40.f;
 constexpr uint32_t kPpGroup = 8;  // parts of an item that one CTA joins by itself
 constexpr int kPpScaleRing = 4, kPpScales = 9;
 
@@ -191,19 +187,24 @@ __device__ __forceinline__ void split(float (&x)[N], uint32_t (&w)[PARTS][N / 4]
         }
     }
 }
-// The same for weights, which are not negative, in a third of the time: they come times 2^-8 (kPpHalf), where the exponent field of a binary16
-// value is that of its e4m3 code, subnormals included, so that the code is the value's bits 14 .. 7.  Each term but the last is cut off there,
-// what remains is exact, and the last is rounded (half up): two terms are off by 2^-8 of the weight at most, three hold the binary16 value.
-// (Rounding the first of two as well, which needs the second's signs, halves that and takes 2 to 4 % longer.)
+// The same for weights, which are not negative, in a third of the time and with more range: the first term is e4m3, those after it are e5m2 (the instruction
+// descriptor of each product says which), whose grid ends at 2^-16 where e4m3's ends at 2^-9.  Weights come times 2^-8 (kPpHalf), where the
+// exponent field of a binary16 value is that of its e4m3 code, subnormals included, so that the rounded value's bits 14 .. 7 are the code.  What remains,
+// exact, is taken back times 2^8, where its upper byte is its e5m2 code, sign included.  The last term is rounded, halves up for odd keys and
+// down for even ones (small weights have few bits left and are often halves: all up, 4096 keys under one of nine tenths of the weight came out 0.0002 too
+// large), one between is cut.  Off by
+// 2^-8 of a weight from 2^-6 up, 2^-14 below (two terms); 2^-11, 2^-17 (three).
 template <int PARTS>
 __device__ __forceinline__ void split_weights(const float *x, uint32_t (&w)[PARTS]) { // of four
-    uint32_t h0 = pack_half2(x[0], x[1]), h1 = pack_half2(x[2], x[3]);
-#pragma unroll
-    for (int p = 0; p < PARTS; p++) {
-        const uint32_t r = p + 1 == PARTS ? 0x00800080u : 0u;
-        w[p] = prmt(h0 * 2 + r, h1 * 2 + r, 0x7531); // the codes stand in the upper bytes
-        if (p + 1 < PARTS) h0 = hsub2_u32(h0, h0 & 0xff80ff80u), h1 = hsub2_u32(h1, h1 & 0xff80ff80u);
+    const uint32_t h0 = pack_half2(x[0], x[1]), h1 = pack_half2(x[2], x[3]);
+    const uint32_t t0 = (h0 + 0x00400040u) & 0xff80ff80u, t1 = (h1 + 0x00400040u) & 0xff80ff80u;
+    w[0] = prmt(t0 * 2, t1 * 2, 0x7531); // the codes stand in the upper bytes
+    uint32_t r0 = hmul2_u32(hsub2_u32(h0, t0), 0x5c005c00u), r1 = hmul2_u32(hsub2_u32(h1, t1), 0x5c005c00u); // times 256
+    if (PARTS == 3) {
+        w[1] = prmt(r0, r1, 0x7531);
+        r0 = hsub2_u32(r0, r0 & 0xff00ff00u), r1 = hsub2_u32(r1, r1 & 0xff00ff00u);
     }
+    w[PARTS - 1] = prmt(r0 + 0x0080007fu, r1 + 0x0080007fu, 0x7531);
 }
 // A bounded wait of a whole warp, in as few instructions as it takes (there are forty of them): polls that the hardware holds for up to a
 // millisecond each, 2000 at most.
@@ -426,7 +427,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             }
         } else {
             // ------------------------------------------------------------ value products
-            constexpr uint32_t idesc = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24);
+            constexpr uint32_t idesc = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kPpRows >> 4) << 24), a_e5m2 = 1u << 7;
             const uint32_t bd0 = uniform(desc_low(smem_u32(ring_v), kPpKeys * 128)), to = uniform(tmem_o), tp = uniform(tmem_p);
             uint32_t g = 0;
             for (uint32_t ni = 0;; ni++) {
@@ -460,7 +461,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t k = 0; k < PARTS * kPpKeys / 32; k++) // 32 keys of one term
-                            tc_mma8_ts(to, ap + k * 8, bd + (k & 3) * 256, idesc, k ? 1u : kt - kt0);
+                            tc_mma8_ts(to, ap + k * 8, bd + (k & 3) * 256, k < kPpKeys / 32 ? idesc : idesc | a_e5m2, k ? 1u : kt - kt0);
                         tc_commit(&pv_done[g & 1]);
                         tc_commit(&v_empty[st]);
                         tc_commit(&sc_empty[ss]); // (its softmax is over too)
@@ -551,7 +552,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 hi = fmaxf(hi, top);
                 const float low = fmaxf(top + kPpSpare, hi - kPpReach);
                 const bool down = low < was - kPpFall && top > -INFINITY;
-                if (!__any_sync(0xffffffffu, top > was + kPpRescale<PARTS> || down)) return was;
+                if (!__any_sync(0xffffffffu, top > was + kPpRescale || down)) return was;
                 return down ? low : fmaxf(was, top + kPpSpare);
             };
             for (uint32_t kt = kt0; kt < kt1; kt++, g++) {
@@ -626,7 +627,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     }
                     tmem_wait_st();
                 }
-                const float base = kPpShift<PARTS> + kPpHalf - (m == -INFINITY ? 0.f : m);
+                const float base = kPpShift + kPpHalf - (m == -INFINITY ? 0.f : m);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int h = 0; h < 3; h++) {
