@@ -246,7 +246,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     qf[nt][ks][1] = pack_half2(x[c][4 * h + 2] * up, x[c][4 * h + 3] * up);
                 }
             }
-            const float undo = __uint_as_float(uint32_t(127 + e) << 23) * a.scale_log2;
+            // (an infinity in a row makes its scores NaN, whatever the keys' signs: all of them -infinity would look like a row without keys)
+            const float undo = top < INFINITY ? __uint_as_float(uint32_t(127 + e) << 23) * a.scale_log2 : __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 rs[nt][j] = __shfl_sync(0xffffffffu, undo, (2 * t + j) * 4);

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import saetta_macqwen_b200 as sa
-from paged_values import Sequences, bf16
+from paged_values import Sequences, bf16, off
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,22 @@ def test_a_later_block_of_large_values_leaves_the_rows_before_it_alone(q_dt, dou
     lim = np.linalg.norm(absv * (2.0 ** -7 + 1e-4) + 2.0 ** (-12 if parts(q_dt) == 2 else -15) * edge, axis=-1)
     err = np.linalg.norm(got - want, axis=-1)
     assert (err <= lim).all(), (err / lim).max()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 24])
+@pytest.mark.parametrize("q_dt", [sa.F32, sa.BF16, sa.F16])
+@pytest.mark.parametrize("kv,sign", [(1, 1.0), (1, -1.0), (40, -1.0)])
+def test_an_infinite_query_gives_nan_whatever_the_keys_signs(rows, q_dt, kv, sign):
+    """All scores at minus infinity are not a row without keys; rows beside it, and rows that see no key, stay as they are."""
+    rng = np.random.default_rng(3)
+    q, k, v = plain(rng, rows, kv)
+    k[..., 5] = np.abs(k[..., 5]) + 1
+    q[:, 3, 5] = sign * np.inf
+    s = Sequences([(q, k, v)], 16, q_dt, DIM ** -0.5)
+    got = s.run()
+    s.q[0][:, 3, 5] = 0
+    want = s.exact()[0]
+    sees = np.arange(rows) >= rows - kv
+    assert np.isnan(got[sees, 3]).all() and (got[~sees] == 0).all()
+    rest = [h for h in range(HEADS) if h != 3]
+    assert off(got[:, rest], want[:, rest]) < 2.0 ** -7
