@@ -374,6 +374,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         pb[u][nt][1] = movmatrix_trans(pack_half2(p[2] * vr, p[3] * vr));
                     }
                 }
+                if (edge && it.lim0 < vis) {
+                    // The tokens see different keys of this piece, and a weight of 0 does not silence NaN: its dims become NaN in the rows that see the key, and 0
+                    // in shared memory (which this warp alone reads) for the products of all.
+#pragma unroll 1
+                    for (int32_t j = max(it.lim0, key0); j < min(vis, key0 + 16 * U); j++) {
+                        const uint32_t at = sub * U * 16 + uint32_t(j - key0), page = at / bt, row = at % bt;
+                        if (scl[st * L::kPages + page].x < 0.f) continue; // of a bad block
+#pragma unroll
+                        for (int sl = 0; sl < kSlabs; sl++) {
+                            const uint32_t addr = smem_u32(ring) + st * L::kStage + L::kSide + page * bt * D + sl * bt * 128 + row * 128 + ((gi ^ (row & 7)) << 4);
+                            const uint4 v = lds128(addr);
+                            uint32_t w[4] = {v.x, v.y, v.z, v.w}, nan[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) nan[e] = (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; // the codes 0x7f and 0xff
+                            if (!__any_sync(0xffffffffu, nan[0] | nan[1] | nan[2] | nan[3])) continue;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+#pragma unroll
+                                for (int b = 0; b < 4; b++)
+#pragma unroll
+                                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                        for (int c = 0; c < 2; c++) // dim 16 gi + 4 e + b of row 2 t + c
+                                            if ((nan[e] >> 8 * b & 1) && j < lim[nt][c]) o[nt][sl * 8 + 2 * e + (b >> 1)][2 * (b & 1) + c] = __uint_as_float(0x7fc00000u);
+                                w[e] &= ~(nan[e] * 255u);
+                            }
+                            if (t == 0) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                            fence_async_smem(); // (the next tile is copied here)
+                            __syncwarp();
+                        }
+                    }
+                }
                 const bool tail = key0 + 16 * U > vis || !all_used; // what lies behind the last key is any byte, NaN too: no product may read it
 #pragma unroll
                 for (int u = 0; u < U; u++)

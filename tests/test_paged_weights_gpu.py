@@ -111,3 +111,41 @@ def test_an_infinite_query_gives_nan_whatever_the_keys_signs(rows, q_dt, kv, sig
     assert np.isnan(got[sees, 3]).all() and (got[~sees] == 0).all()
     rest = [h for h in range(HEADS) if h != 3]
     assert off(got[:, rest], want[:, rest]) < 2.0 ** -7
+
+
+NANS = [  # few rows; heads, dim, block, keys, rows, the keys that hold NaN
+    (2, 128, 16, 6, 6, [2, 4]),
+    (2, 128, 16, 300, 8, [295, 298]),
+    (4, 256, 64, 130, 4, [127, 129]),
+    (8, 256, 32, 700, 2, [699]),
+    (1, 128, 128, 200, 16, [190, 199]),
+    (8, 128, 16, 5000, 2, [10, 4999]),
+    (3, 256, 64, 64, 5, [60, 62]),
+]
+
+
+@pytest.mark.parametrize("q_dt", [sa.BF16, sa.F16])
+@pytest.mark.parametrize("heads,dim,block,kv,rows,keys", NANS)
+def test_nan_reaches_the_rows_that_see_it_and_no_other(q_dt, heads, dim, block, kv, rows, keys):
+    """NaN in a few dims of some rows' values, the others' among the same keys: in the dims that have it for the rows that see the key, and
+    nowhere for those before it.  The same for a NaN key, which takes the whole row."""
+    rng = np.random.default_rng(kv + rows)
+    for side in (2, 1):
+        x = list(plain(rng, rows, kv, dim=dim, heads=heads))
+        for i, key in enumerate(keys):
+            x[side][key, 0, [3 + i, dim - 1]] = np.nan
+        s = Sequences([tuple(x)], block, q_dt, dim ** -0.5, seed=kv)
+        got = s.run()
+        for i in range(2):
+            s.kv[i][0] = np.nan_to_num(s.kv[i][0])
+        want = s.exact()[0]
+        nan = np.zeros(want.shape, bool)
+        for i, key in enumerate(keys):
+            sees = np.arange(rows) + kv - rows >= key
+            if side == 1:
+                nan[sees] = True
+            else:
+                nan[np.ix_(sees, np.arange(heads), [3 + i, dim - 1])] = True
+        assert np.array_equal(np.isnan(got), nan), np.argwhere(np.isnan(got) != nan)[:5]
+        err = np.abs(np.where(nan, 0, got - want)).max((1, 2))
+        assert (err < 2.0 ** -5).all(), err.max()
