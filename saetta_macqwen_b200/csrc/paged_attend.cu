@@ -15,8 +15,8 @@
 //    swizzle, chunk 2 t + j for lane t of a key makes these 128-bit loads free of bank conflicts, and chunk g for lane
 //    group g those of the values.
 //  * Values enter as pairs of keys of one dim: two byte permutes for four dims, then the conversion to binary16.
-//  * P is rounded to binary16 (11 bits; p times the value scale relative to the largest of the warp's so far), scores, sums
-//    and accumulators are f32.  Queries enter as binary16 after a power of two for each row, so bfloat16's range
+//  * P is rounded to binary16 (11 bits; with the value scale in it, relative to the largest of the warp's so far; the maximum it stands against is of both, over the
+//    keys that the row sees), scores, sums and accumulators are f32.  Queries enter as binary16 after a power of two for each row, so bfloat16's range
 //    fits; f32 queries are rounded to 11 bits there.
 //
 // Measured: one sequence of 131072 keys (bfloat16, 16 query and 2 kv heads of 256) 40 us (3.4 TB/s; the bytes alone take 20.5), 61 sequences of up to
@@ -24,6 +24,7 @@
 // first pages, the first bytes: 6 us), the change of items, and the parts' joining (3 to 4 us a round).  (One warp for keys, values and scales together: 61 sequences 139 us; copies issued page
 // by page from one lane: 173; scores of two products for 32 rows in place of the many-rows kernel: 138 against 96.)
 #include <algorithm>
+#include <cfloat>
 
 #include "paged_sched.cuh"
 #include "umma.cuh"
@@ -34,6 +35,7 @@ constexpr int kPdThreads = 384;  // 8 consumer warps; items and keys, values, sc
 constexpr uint32_t kPdGroup = 12; // parts of an item that one CTA joins by itself; one more in each of two rounds
 static_assert((kPdGroup + 1) * (kPdGroup + 1) >= uint32_t(kPagedMaxCtas), "two rounds join the parts of every CTA");
 constexpr float kPdRescale = 8.f; // the accumulators follow the running maximum only past this many doublings
+constexpr float kPdShift = 7.f;   // weights are kept times this many doublings: binary16 ends at 2^16, and is whole down to 2^-14
 
 template <int D, int NT>
 struct PdLayout {
@@ -313,15 +315,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 bool all_used = true;
 #pragma unroll
                 for (int u = 0; u < U; u++) vnew = fmaxf(vnew, sc[u].y), all_used &= use[u];
+                vnew = fmaxf(vnew, FLT_MIN);
                 float s[U][NT][4];
                 uint32_t pb[U][NT][2];
                 bool need = vnew != vref;
-                float f[NT][2];
+                float f[NT][2], d[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) d[u] = fmaxf(lg2_approx(sc[u].y / vnew), -60.f);
+                // A larger value scale: O keeps its place by the maximum's falling as much, so far as the sum l, which has no r in it, can follow.
+                const float up = need && vref > 0.f ? lg2_approx(vnew / vref) : 0.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         float mx = -INFINITY;
+                        f[nt][j] = 1.f;
+                        if (up > 0.f) {
+                            const float by = fminf(up, float(max(0, 227 - max(127, int(__float_as_uint(l[nt][j]) >> 23))))); // l stays below 2^101
+                            m[nt][j] -= by, l[nt][j] *= ex2_approx(by), f[nt][j] = ex2_approx(by - up);
+                        }
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             const float c = sc[u].x * rs[nt][j];
@@ -329,7 +341,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             for (int k = 0; k < 2; k++) { // key gi, key gi + 8
                                 float x = acc[u][0][nt][2 * k + j] + acc[u][1][nt][2 * k + j];
                                 if (kChains == 4) x += acc[u][kChains - 2][nt][2 * k + j] + acc[u][kChains - 1][nt][2 * k + j];
-                                x *= c;
+                                x = fmaf(x, c, d[u]); // of what the key puts into O: the value scale is in it
                                 if ((edge && key0 + u * 16 + int32_t(gi) + 8 * k >= lim[nt][j]) || !use[u]) x = -INFINITY;
                                 s[u][nt][2 * k + j] = x;
                                 mx = fmaxf(mx, x);
@@ -338,40 +350,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        f[nt][j] = 1.f;
                         if (mx > m[nt][j] + kPdRescale) {
-                            f[nt][j] = ex2_approx(m[nt][j] - mx); // 0 for the first
+                            const float g1 = ex2_approx(m[nt][j] - mx); // 0 for the first
                             m[nt][j] = mx;
-                            l[nt][j] *= f[nt][j];
+                            l[nt][j] *= g1, f[nt][j] *= g1;
                             need = true;
                         }
                     }
                 }
                 if (__any_sync(0xffffffffu, need)) {
-                    const float fv = vnew > 0.f ? vref / vnew : 1.f;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int i = 0; i < kSlabs * 8; i++) {
-                            o[nt][i][0] *= f[nt][0] * fv, o[nt][i][1] *= f[nt][1] * fv;
-                            o[nt][i][2] *= f[nt][0] * fv, o[nt][i][3] *= f[nt][1] * fv;
+                            o[nt][i][0] *= f[nt][0], o[nt][i][1] *= f[nt][1];
+                            o[nt][i][2] *= f[nt][0], o[nt][i][3] *= f[nt][1];
                         }
                     vref = vnew;
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const float vr = vref > 0.f ? sc[u].y / vref : 0.f;
+                    const float ir = ex2_approx(-d[u]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         float p[4];
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
-                            const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+                            const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j] - kPdShift;
                             p[j] = ex2_approx(s[u][nt][j] - mu), p[2 + j] = ex2_approx(s[u][nt][2 + j] - mu);
-                            l[nt][j] += p[j] + p[2 + j];
+                            l[nt][j] = fmaf(p[j] + p[2 + j], ir, l[nt][j]);
                         }
-                        pb[u][nt][0] = movmatrix_trans(pack_half2(p[0] * vr, p[1] * vr));
-                        pb[u][nt][1] = movmatrix_trans(pack_half2(p[2] * vr, p[3] * vr));
+                        pb[u][nt][0] = movmatrix_trans(pack_half2(p[0], p[1]));
+                        pb[u][nt][1] = movmatrix_trans(pack_half2(p[2], p[3]));
                     }
                 }
                 if (edge && it.lim0 < vis) {
@@ -451,7 +461,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             float top = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; k++) top = fmaxf(top, wm[k * R + row]);
-            const float mu = top == -INFINITY ? 0.f : top;
+            const float mu = (top == -INFINITY ? 0.f : top) + kPdShift; // the parts' values are without it
 #pragma unroll
             for (int k = 0; k < 8; k++) sum += wl[k * R + row] * ex2_approx(wm[k * R + row] - mu);
             ww[w * R + row] = ex2_approx(wm[w * R + row] - mu) * wv[w];

@@ -225,11 +225,6 @@ __device__ __forceinline__ uint32_t in_order(float x) {
     return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float(u ^ (uint32_t(int32_t(~u) >> 31) | 0x80000000u)); }
-__device__ __forceinline__ float lg2_approx(float x) {
-    float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 template <int D, int PARTS>
 __global__ void __launch_bounds__(kPpThreads, 1)

@@ -275,6 +275,11 @@ __device__ __forceinline__ void paged_store4(const PagedArgs &a, size_t i, float
             make_uint2(*reinterpret_cast<const uint32_t *>(&p), *reinterpret_cast<const uint32_t *>(&r));
     }
 }
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
 // 8 consecutive values of q.

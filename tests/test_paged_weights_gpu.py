@@ -149,3 +149,24 @@ def test_nan_reaches_the_rows_that_see_it_and_no_other(q_dt, heads, dim, block, 
         assert np.array_equal(np.isnan(got), nan), np.argwhere(np.isnan(got) != nan)[:5]
         err = np.abs(np.where(nan, 0, got - want)).max((1, 2))
         assert (err < 2.0 ** -5).all(), err.max()
+
+
+@pytest.mark.parametrize("dim,q_dt", [(128, sa.F16), (256, sa.BF16)])
+@pytest.mark.parametrize("doublings,nats,share", [(10, -40, 0), (20, -40, 0), (40, -80, 0), (60, -80, 0), (-140, 0, 0), (0, 0, 0.99), (0, 0, 0.9999)])
+def test_long_shares_of_a_decode_batch(dim, q_dt, doublings, nats, share):
+    """So many sequences that a warp goes through several tiles of each: a block of large values and little weight, zeros, or a first key of
+    much weight takes nothing from what the warp meets after it."""
+    rng = np.random.default_rng(dim + 200 + doublings)
+    seqs = []
+    for i in range(37):
+        kv = int(rng.integers(2500, 4500))
+        q, k, v = plain(rng, 2, kv, dim=dim)
+        at = 64 * int(rng.integers(0, 4))
+        k[at:at + 64, 0, 0] = nats * dim ** 0.5
+        v[at:at + 64] *= 2.0 ** doublings if doublings > -100 else 0
+        if share:
+            k[0], v[0] = 0, rng.normal(size=dim) * 0.01
+            k[0, 0, 0] = np.log(kv * np.exp(0.5) * share / (1 - share)) * dim ** 0.5
+        seqs.append((q, k, v))
+    s = Sequences(seqs, 64, q_dt, dim ** -0.5)
+    near(s, s.run())
