@@ -564,7 +564,7 @@ int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *ca
     PagedArgs a{};
     a.q = q_dev, a.q_and_gate = q_and_gate_dev, a.out = out_dev;
     a.row_starts = batch.row_starts_dev, a.kv_lens = batch.kv_lens_dev, a.tables = batch.block_tables_dev;
-    a.scales = cache->scales, a.parts = op->parts, a.words = op->words, a.part_floats = op->part_floats;
+    a.scales = cache->scales, a.parts = op->parts, a.words = op->words, a.values = cache->values, a.part_floats = op->part_floats;
     a.q_stride = uint32_t(q_stride), a.rows = uint32_t(batch.rows), a.seqs = uint32_t(batch.seqs);
     a.table_stride = uint32_t(batch.table_stride), a.blocks = uint32_t(cache->blocks);
     a.heads = uint32_t(op->heads), a.kv_heads = uint32_t(op->kv_heads), a.group = uint32_t(op->heads / op->kv_heads);

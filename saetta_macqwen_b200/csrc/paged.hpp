@@ -47,6 +47,7 @@ struct PagedArgs {
     const float *scales;
     float *parts;
     uint32_t *words;
+    const uint8_t *values;
     size_t part_floats;
     uint32_t q_stride; // values between the rows of q
     uint32_t rows, seqs, table_stride, blocks;

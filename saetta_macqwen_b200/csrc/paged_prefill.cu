@@ -206,6 +206,11 @@ __device__ __forceinline__ void split_weights(const float *x, uint32_t (&w)[PART
     }
     w[PARTS - 1] = prmt(r0 + 0x0080007fu, r1 + 0x0080007fu, 0x7531);
 }
+// Each byte of four codes that is NaN (0x7f or 0xff) as 0xff, the others as 0.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 255u; }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 // A bounded wait of a whole warp, in as few instructions as it takes (there are forty of them): polls that the hardware holds for up to a
 // millisecond each, 2000 at most.
 __device__ __forceinline__ bool short_wait(uint64_t *bar, uint32_t parity) {
@@ -250,6 +255,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
              *all_met = s_free + 3, *x_met = s_free + 4 /* [4 tiles][4 row quarters] */;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(x_met + 16);
     volatile uint32_t *never_set = tmem_slot + 1, *arrived = tmem_slot + 2;
+    volatile uint32_t *nan_item = tmem_slot + 3; // bit ni & 1: item ni has NaN in values that some of its rows do not see (set before o_final)
     uint8_t *row_e = reinterpret_cast<uint8_t *>(tmem_slot + 4); // [128]: the power of two (biased) that undoes what a row of Q was scaled by
 
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -265,9 +271,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int s = 0; s < kPpItems; s++) mbar_init(&item_full[s], 1), mbar_init(&item_empty[s], kPpItemReaders);
         for (int s = 0; s < 2; s++) mbar_init(&s_full[s], 2), mbar_init(&p_full[s], kPpWarps / 2), mbar_init(&pv_done[s], 1);
         for (int s = 0; s < 16; s++) mbar_init(&x_met[s], 2);
-        mbar_init(q_full, 4), mbar_init(q_empty, 1 + kPpWarps), mbar_init(s_free, kPpWarps / 2), mbar_init(o_final, 1), mbar_init(o_empty, kPpWarps);
+        mbar_init(q_full, 4), mbar_init(q_empty, 1 + kPpWarps), mbar_init(s_free, kPpWarps / 2), mbar_init(o_final, 2), mbar_init(o_empty, kPpWarps);
         mbar_init(all_met, kPpWarps);
-        *never_set = 0;
+        *never_set = 0, *nan_item = 0;
         mbar_fence_init();
     }
     pdl_wait();
@@ -429,6 +435,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 PP_WAIT(&item_full[ni % kPpItems], ni / kPpItems & 1);
                 const int32_t keys = int32_t(items[ni % kPpItems].keys);
                 const uint32_t kt0 = uniform(items[ni % kPpItems].kt0), kt1 = uniform(items[ni % kPpItems].kt1);
+                const int32_t lim0 = items[ni % kPpItems].lim0;
+                uint32_t nan_found = 0;
                 if (kt0 == kt1) break;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
@@ -439,14 +447,45 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     // rows behind the last key, and of bad blocks, may hold NaN, which a weight of 0 does not silence
                     const int32_t key0 = int32_t(kt * kPpKeys);
                     const uint32_t bad = __ballot_sync(0xffffffffu, lane < 8 && scl[ss * kPpScales + (lane & 7)].x < 0.f);
+                    const uint32_t tile = smem_u32(ring_v) + st * L::kStage;
                     if (key0 + kPpKeys > keys || bad) {
-                        for (uint32_t k = lane; k < kPpKeys * 8 * kSlabs; k += 32) {
-                            const uint32_t key = (k >> 3) % kPpKeys, slab = k / (kPpKeys * 8);
-                            if (key0 + int32_t(key) >= keys || (bad >> (key >> 4) & 1))
-                                *reinterpret_cast<uint4 *>(ring_v + st * L::kStage + slab * (kPpKeys * 128) + key * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+                        for (uint32_t slab = 0; slab < kSlabs; slab++) {
+                            const uint32_t end = tile + (slab + 1) * (kPpKeys * 128);
+#pragma unroll 1
+                            for (uint32_t at = end - kPpKeys * 128 + lane * 16, key = lane >> 3; bad && at < end; at += 512, key += 4)
+                                if (bad >> (key >> 4) & 1) sts128(at, 0, 0, 0, 0);
+#pragma unroll 1
+                            for (uint32_t at = end - min(uint32_t(key0 + kPpKeys - keys), 128u) * 128 + lane * 16; key0 + kPpKeys > keys && at < end; at += 512) sts128(at, 0, 0, 0, 0);
                         }
                         fence_async_smem();
                         __syncwarp();
+                    }
+                    if (lim0 < keys && key0 + kPpKeys > lim0) {
+                        // Keys that some rows do not see, and a weight of 0 does not silence NaN either: it becomes 0 to the products, and NaN again at the tile's end in
+                        // the rows that see the key.
+                        const uint32_t hi = tile + uint32_t(min(keys - key0, kPpKeys)) * 128;
+                        bool found = false;
+#pragma unroll
+                        for (uint32_t slab = 0; slab < kSlabs; slab++)
+#pragma unroll 2
+                            for (uint32_t at = tile + uint32_t(max(lim0 - key0, 0)) * 128 + lane * 16; at < hi; at += 512) {
+                                const uint4 v = lds128(at + slab * (kPpKeys * 128));
+                                const uint32_t x = nan_codes(v.x), y = nan_codes(v.y), z = nan_codes(v.z), w = nan_codes(v.w);
+                                if (x | y | z | w) {
+                                    sts128(at + slab * (kPpKeys * 128), v.x & ~x, v.y & ~y, v.z & ~z, v.w & ~w);
+                                    found = true;
+                                }
+                            }
+                        if (__any_sync(0xffffffffu, found)) {
+                            fence_async_smem();
+                            __syncwarp();
+                            nan_found = 1;
+                        }
+                    }
+                    if (kt + 1 == kt1 && lane == 0) {
+                        *nan_item = (*nan_item & ~(1u << (ni & 1))) | nan_found << (ni & 1);
+                        mbar_arrive(o_final);
                     }
                     if (kt == kt0) PP_WAIT(o_empty, (ni & 1) ^ 1);
                     PP_WAIT(&p_full[pb], g / NP & 1);
@@ -688,8 +727,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const uint32_t c0 = it.span & 0xffff, parts = it.span >> 16;
             const size_t orow = live ? size_t(it.row0 + tok) * a.heads + it.head * a.group + hq : 0;
             const float vref = it.vref;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
             PP_WAIT(o_final, ni & 1);
             tc_fence_after();
             auto finish = [&](int d, float4 v, float inv) { // dims d .. d + 3 of this thread's row
@@ -723,6 +760,25 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     }
                 }
             }
+            if (*nan_item >> (ni & 1) & 1) { // dims that some rows see as NaN
+                const uint32_t bt = a.block_tokens;
+                const int32_t end = min(lim, int32_t(min(it.keys, kt1 * kPpKeys)));
+#pragma unroll 1
+                for (int32_t key = max(lim0, int32_t(kt0 * kPpKeys)); live && key < end; key++) {
+                    const uint32_t block = uint32_t(a.tables[size_t(it.seq) * a.table_stride + uint32_t(key) / bt]);
+                    if (block >= a.blocks) continue;
+                    const uint8_t *code = a.values + ((size_t(block) * a.kv_heads + it.head) * bt + uint32_t(key) % bt) * D;
+#pragma unroll 1
+                    for (uint32_t d = cq * (D / 4); d < (cq + 1) * (D / 4); d++) {
+                        if ((code[d] & 0x7f) != 0x7f) continue;
+                        if (parts > 1) part[size_t(row) * D + d] = __uint_as_float(0x7fc00000u);
+                        else if (a.out_dtype == SAETTA_F32) static_cast<uint32_t *>(a.out)[orow * D + d] = 0x7fc00000u;
+                        else static_cast<uint16_t *>(a.out)[orow * D + d] = a.out_dtype == SAETTA_F16 ? 0x7e00 : 0x7fc0;
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[ni % kPpItems]);
             if (parts > 1) {
                 if (cq == 0) *reinterpret_cast<float2 *>(part + kPpRows * D + row * 2) = make_float2(m, l);
                 if (warp == 0 && lane == 0) part[kPpRows * (D + 2)] = vref;

@@ -121,6 +121,14 @@ NANS = [  # few rows; heads, dim, block, keys, rows, the keys that hold NaN
     (1, 128, 128, 200, 16, [190, 199]),
     (8, 128, 16, 5000, 2, [10, 4999]),
     (3, 256, 64, 64, 5, [60, 62]),
+    # many rows
+    (8, 128, 16, 200, 200, [0, 50, 130]),
+    (2, 256, 64, 300, 70, [231, 299, 257]),
+    (1, 128, 32, 700, 400, [300, 511, 512, 600, 699]),
+    (16, 256, 128, 1000, 40, [961, 999, 5]),
+    (8, 128, 64, 9000, 20, [8981, 8999, 4000]),
+    (3, 128, 16, 50, 90, [10, 49]),
+    (12, 256, 16, 130, 130, [126, 127, 128, 129]),
 ]
 
 
