@@ -591,7 +591,9 @@ int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *ca
                         const float *q_and_gate_dev, void *out_dev, int out_dtype, float scale,
                         void *stream);
 /* The op's device status word: 0, or bits of a bounded wait that gave up (1, 2, 4: make a new
- * op) or of a block table entry outside the cache (16: that block's keys were left out).
+ * op), of a block table entry outside the cache (16: that block's keys were left out), or of
+ * a length that the call cut off (32: kv_lens behind its row of the block table, row_starts
+ * behind `rows` or falling).
  * Synchronises the stream. */
 int saetta_paged_attention_status(saetta_paged_attention *op, void *stream, uint32_t *status);
 

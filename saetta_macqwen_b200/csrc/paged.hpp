@@ -25,6 +25,7 @@ struct saetta_paged_attention {
 namespace saetta {
 
 constexpr uint32_t kStatusBadBlock = 16u; // a block table entry outside the cache was met
+constexpr uint32_t kStatusCut = 32u;      // a length behind its row of the block table, or rows behind the call's, were cut off
 constexpr int kPagedBadScale = 2;         // word index of the (-1, -1) pair
 constexpr int kPagedCounters = 8;
 constexpr int kPagedMaxGroup = 16;        // query heads of one kv head

@@ -68,3 +68,26 @@ def test_assign_of_every_number_of_sequences_in_a_process_that_made_no_larger_ca
     here = os.path.dirname(os.path.abspath(__file__))
     r = subprocess.run([sys.executable, "-c", FRESH.format(path=[here, os.path.dirname(here)])], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_lengths_that_are_cut_off_are_reported(rows):
+    """A length behind its row of the block table, rows behind the call's, falling row starts: cut off as before, and said."""
+    import torch
+
+    from test_paged_gpu import i32
+
+    def run(change):
+        c = Case(16, 2, 256, 16, [(90, rows), (64, rows)], sa.BF16, sa.F32, seed=2)
+        change(c)
+        op = c.op()
+        c.record(op)
+        torch.cuda.synchronize()
+        return op.device_status()
+
+    assert run(lambda c: None) == 0
+    longest = lambda c: c.dev.__setitem__(3, i32([90, c.width * 16]))  # noqa: E731 (its last pages lie outside the cache)
+    assert run(longest) & 32 == 0
+    assert run(lambda c: c.dev.__setitem__(3, i32([90, c.width * 16 + 1]))) & 32
+    assert run(lambda c: c.dev.__setitem__(2, i32([0, rows, 2 * rows + 1]))) & 32
+    assert run(lambda c: c.dev.__setitem__(2, i32([0, rows, rows - 1]))) & 32
