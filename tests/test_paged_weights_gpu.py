@@ -178,3 +178,24 @@ def test_long_shares_of_a_decode_batch(dim, q_dt, doublings, nats, share):
         seqs.append((q, k, v))
     s = Sequences(seqs, 64, q_dt, dim ** -0.5)
     near(s, s.run())
+
+
+@pytest.mark.parametrize("dim,q_dt", [(128, sa.F16), (128, sa.BF16), (256, sa.F16), (256, sa.BF16)])
+@pytest.mark.parametrize("doublings,nats,share", [(10, -40, 0), (40, -80, 0), (-140, 0, 0), (0, 0, 0.9), (0, 700, 0), (0, -30, 0), (-20, 0, 0)])
+def test_long_shares_of_prompts(dim, q_dt, doublings, nats, share):
+    """The same for the many-rows kernel: so many prompts that a CTA goes through all tiles of a row tile, and its weights' reference goes up and
+    down on the way: 192 keys of other scores and values, or a first key of much weight."""
+    rng = np.random.default_rng(dim + 300 + doublings + int(share * 10))
+    seqs = []
+    for i in range(30):
+        kv = int(rng.integers(900, 1700))
+        q, k, v = plain(rng, 32, kv, dim=dim)
+        at = 64 * int(rng.integers(0, 8))
+        k[at:at + 192, 0, 0] = nats * dim ** 0.5
+        v[at:at + 192] *= 2.0 ** doublings if doublings > -100 else 0
+        if share:
+            k[0], v[0] = 0, rng.normal(size=dim) * 0.01
+            k[0, 0, 0] = np.log(kv * np.exp(0.5) * share / (1 - share)) * dim ** 0.5
+        seqs.append((q, k, v))
+    s = Sequences(seqs, 64, q_dt, dim ** -0.5)
+    near(s, s.run())
