@@ -40,6 +40,8 @@ constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the va
 // it; now in one of ten.)
 constexpr float kPpShift = 6.f, kPpRescale = 2.5f;
 constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 1.f, kPpFall = 8.f, kPpReach = 40.f;
+// Largest |log2 of a weight| that f32 holds to an eighth: past it the difference to the maximum, in one FMA, may pass what a first term holds.  Such rows get NaN.
+constexpr float kPpMaxScore = 1048576.f;
 constexpr uint32_t kPpGroup = 8;  // parts of an item that one CTA joins by itself
 constexpr int kPpScaleRing = 4, kPpScales = 9;
 
@@ -720,6 +722,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             lx[(team * 2 + half) * 128 + row] = l;
             PP_MEET_ALL();
             l = ((lx[row] + lx[128 + row]) + (lx[256 + row] + lx[384 + row])) * 256.f; // (the weights' sums were taken times 2^-8)
+            if (fabsf(hi) > kPpMaxScore && hi > -INFINITY) l = __uint_as_float(0x7fc00000u);
             PP_MEET_ALL();
             const PpItem &it = items[ni % kPpItems];
             const uint32_t cq = warp >> 2, tok = row / a.group, hq = row % a.group;

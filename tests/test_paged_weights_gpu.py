@@ -199,3 +199,24 @@ def test_long_shares_of_prompts(dim, q_dt, doublings, nats, share):
         seqs.append((q, k, v))
     s = Sequences(seqs, 64, q_dt, dim ** -0.5)
     near(s, s.run())
+
+
+@pytest.mark.parametrize("rows,kernel", ROWS)
+@pytest.mark.parametrize("q_dt", [sa.BF16, sa.F16, sa.F32])
+@pytest.mark.parametrize("size,nan", [(2.0 ** 12, False), (2.0 ** 24, True), (2.0 ** 34, True)])
+def test_scores_past_what_f32_resolves(rows, kernel, q_dt, size, nan):
+    """One key's score stands out by far.  Up to 2^20 both kernels return its value; past that a difference of two scores has no fraction left: the few-rows
+    kernel still does, the many-rows kernel returns NaN and never another key's value."""
+    rng = np.random.default_rng(4)
+    q, k, v = plain(rng, rows, 700)
+    k[..., 0] = 1.0
+    k[300, 0, 0] = 1.5
+    q[..., 0] = 2.0 ** 12
+    s = Sequences([(q, k, v)], 64, q_dt, DIM ** -0.5 * size / 2.0 ** 12)
+    got, want = s.run(), np.broadcast_to(s.kv[1][0][0][300], (rows, HEADS, DIM))
+    if nan and kernel == "many":
+        assert np.isnan(got).all()
+    else:
+        # The one weight is 2 to the power of a difference of two f32 numbers of 1.44 * 1.5 * 4096 = 2^13.1, rounded to 2^-10 each, and its sum has what the products'
+        # first term rounds away: off by 2 * 2^-11 * ln 2 < 2^-10 at most.  (The few-rows kernel subtracts after rounding: exact.)
+        assert (np.abs(got - want) <= (2.0 ** -10 * np.abs(want) if kernel == "many" else 0)).all()
