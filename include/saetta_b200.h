@@ -546,8 +546,9 @@ int saetta_paged_assign(int device, size_t seqs, size_t block_tokens, const uint
  * SAETTA_BF16; k_stride, v_stride: values between rows; rows 16-byte aligned) at `slots`; a
  * negative slot is skipped.  Rows of one block stand next to each other in rising order, as
  * assign lays them out, and a slot occurs once: a row of the same block as the one before it
- * but not its successor is not written and reported, as is a slot outside the cache
- * (SAETTA_PAGED_BAD_SLOT is OR-ed into *status_dev, which may be NULL).  Two runs of rows in
+ * but not its successor is not written, nor are those that go on from it, and it is reported, as
+ * is a slot outside the cache (SAETTA_PAGED_BAD_SLOT is OR-ed into *status_dev, which may be
+ * NULL).  Two runs of rows in
  * one block, apart from one another, leave that block undefined.
  * A run that begins at a block's first token starts its scales anew from the run's values; a
  * later one raises them where its values need it and re-scales the tokens before the run.
@@ -583,14 +584,21 @@ void saetta_paged_attention_destroy(saetta_paged_attention *op);
  * [rows][heads][head_dim], q_stride values between rows (at least heads * head_dim), rows
  * 16-byte aligned; q_dtype and out_dtype each SAETTA_F32, SAETTA_F16 or SAETTA_BF16.
  * Scores, sums and accumulators are f32; the products take q with the precision of its type,
- * 11 bits of an f32 one, and the probabilities with 11 bits; with more than 16 rows (tokens x
- * heads of a kv head) and bfloat16 q with 8, and down to 2^-15 of the row's largest.  A row of q
- * with an infinity or a NaN gets NaN.  max_rows below the real count costs time alone. */
+ * 11 bits of an f32 one.  Weights: with up to 16 rows (tokens x heads of a kv head) binary16,
+ * that is 11 bits; with more, 8 bits for bfloat16 q and 11 else, less where a weight (times its
+ * block's value scale) falls below 2^-4 of the largest that the row has among the same 128 keys:
+ * off by 2^-12 (2^-15) of that one at most.  A key of much weight, or a block of larger values
+ * whose keys have little, takes nothing from the keys of other tiles as long as these are within
+ * 2^-40 of it; value scales below 2^-60 of the sequence's largest count as 2^-60 of it.  Scores
+ * may have any common offset; with more than 16 rows a row whose largest score (in log2 units)
+ * passes 2^20 gets NaN.
+ * NaN in a key or a value reaches the rows that see it and no other (a value: in its dim alone).
+ * A row of q with an infinity or a NaN gets NaN.  max_rows below the real count costs time alone. */
 int saetta_paged_attend(saetta_paged_attention *op, const saetta_paged_cache *cache,
                         saetta_paged_batch batch, const void *q_dev, int q_dtype, size_t q_stride,
                         const float *q_and_gate_dev, void *out_dev, int out_dtype, float scale,
                         void *stream);
-/* The op's device status word: 0, or bits of a bounded wait that gave up (1, 2, 4: make a new
+/* The op's device status word: 0, or, from any call so far, bits of a bounded wait that gave up (1, 2, 4: make a new
  * op), of a block table entry outside the cache (16: that block's keys were left out), or of
  * a length that the call cut off (32: kv_lens behind its row of the block table, row_starts
  * behind `rows` or falling).

@@ -49,8 +49,9 @@ __device__ __forceinline__ uint32_t last_at_or_below(const uint32_t *a, uint32_t
 // blocks given back, blocks taken, rows -- into shared memory, and then the cluster's threads deal out table entries and
 // rows, each finding its sequence by a binary search over the sums.  Nothing is written before every CTA has read its
 // inputs (cluster barrier), so lengths and count may be updated in place.  Bound by latency: the chain is lengths ->
-// scan -> free stack -> tables and slots.  1 sequence 2.9 us, 509 sequences of one token each 9, 1024 prompts of 133,000 rows in all 14.5
-// (a cluster of 8 CTAs above 4096 rows: the rows' writes then weigh more than the cluster's start).
+// scan -> free stack -> tables and slots.  1024 prompts of 133,000 rows in all 14.2 us a call, one behind the other (a cluster of 8 CTAs above 4096
+// rows: the rows' writes then weigh more than the cluster's start); 1 sequence and 509 of one token each 10.2, which is the host's call (from
+// cold caches 5.0 and 13.0).
 __global__ void __launch_bounds__(kAssignThreads) paged_assign_kernel(const AssignArgs a) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -242,8 +243,8 @@ __device__ __forceinline__ float pow2_scale(float amax) {
 // A CTA for each (16 rows of the call, kv head, side): it takes the runs (rows of one block, one behind the other) that begin there, long ones with all
 // of its warps, short ones with a warp each; a row leads a run where the row before it lies in another block.  Bound by memory: rows
 // in, codes out, each once (the second pass over a run, which needs its largest value, hits the caches).  17413 bfloat16 rows of 2 x 256
-// in blocks of 64: 15.6 us, 3.4 TB/s (the rows of one launch after the other stay in L2; a run's two passes and their meeting are what is left); a warp for
-// each run took 45: too few loads on their way.  One row 2.0 us, 253 rows of as many sequences 5.1.
+// in blocks of 64: 21.0 us, 2.55 TB/s (a run's two passes and their meeting are what is left); a warp for each run took 45: too few loads on
+// their way.  One row, and 253 rows of as many sequences: 7.9 us, the host's call (from cold caches 4.0 and 7.5 to 8.1).
 template <int DT, int D>
 __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
     constexpr uint32_t kLanes = D / 8;      // lanes of one row

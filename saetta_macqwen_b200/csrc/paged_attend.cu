@@ -19,8 +19,8 @@
 //    keys that the row sees), scores, sums and accumulators are f32.  Queries enter as binary16 after a power of two for each row, so bfloat16's range
 //    fits; f32 queries are rounded to 11 bits there.
 //
-// Measured: one sequence of 131072 keys (bfloat16, 16 query and 2 kv heads of 256) 40 us (3.4 TB/s; the bytes alone take 20.5), 61 sequences of up to
-// 8192 keys (binary16, 32 over 8 heads of 128) 128 us (3.7 TB/s), 701 keys 12.9 us.  What is left beyond the bytes is the start of a CTA (its share, the
+// Measured: one sequence of 131072 keys (bfloat16, 16 query and 2 kv heads of 256) 40.5 us (3.3 TB/s; the bytes alone take 20.5), 61 sequences of up to
+// 8192 keys (binary16, 32 over 8 heads of 128) 125 us (3.8 TB/s), 701 keys 12.6 us.  What is left beyond the bytes is the start of a CTA (its share, the
 // first pages, the first bytes: 6 us), the change of items, and the parts' joining (3 to 4 us a round).  (One warp for keys, values and scales together: 61 sequences 139 us; copies issued page
 // by page from one lane: 173; scores of two products for 32 rows in place of the many-rows kernel: 138 against 96.)
 #include <algorithm>

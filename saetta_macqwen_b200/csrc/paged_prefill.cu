@@ -16,10 +16,10 @@
 // tiles by turns (two threads for each row, 64 keys each), four warps that bring a tile's Q rows, one warp each for the K/V copies, the score
 // products, the scales and the value products.
 //
-// Measured (bfloat16, 16 query and 2 kv heads of 256, 4096 rows at 28672 keys): 1.53 to 1.6 ms in a burst (1.3 PFLOP/s counted as 16-bit
-// products), 1.78 in a stream of calls under the power limit.  With head dim 128 a tile has half the products and the same softmax, which then bounds it: a warp needs 5000
+// Measured (bfloat16, 16 query and 2 kv heads of 256, 4096 rows at 28672 keys): 1.85 ms in a stream of calls under the power limit (1.12 PFLOP/s counted as
+// 16-bit products).  With head dim 128 a tile has half the products and the same softmax, which then bounds it: a warp needs 5000
 // clocks for its tile, two teams so 2600 a tile (1024 of products); binary16 queries 3600 (1536).  7 prompts of 425 to 2554 keys, 32 over 8
-// heads of 128, binary16: 653 us.  Beside the tiles: 14,000 clocks before a CTA's first item (its code and share come cold), 10,000 for the first Q rows (later
+// heads of 128, binary16: 683 us (18 of them so that NaN stays with the rows that see it).  Beside the tiles: 14,000 clocks before a CTA's first item (its code and share come cold), 10,000 for the first Q rows (later
 // ones come under the tiles before), 12,000 between items, up to 24,000 where the last CTA joins an item's parts.  (A second Q buffer, tried
 // for head dim 128: 688 us against 640.  Q rows four at a time, each read by 8 lanes: 900, from spills.)
 #include <algorithm>
@@ -39,7 +39,9 @@ constexpr int kPpAhead = 2;   // keys are copied this many tiles ahead of the va
 // following for itself past 2 doublings, some row of a CTA did so in every other tile of a random prompt of 8192 keys, and the products wait for
 // it; now in one of ten.)
 constexpr float kPpShift = 6.f, kPpRescale = 2.5f;
-constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 1.f, kPpFall = 8.f, kPpReach = 40.f;
+constexpr float kPpHalf = -8.f /* see split_weights */, kPpSpare = 1.f;
+// The reference falls where a tile's largest lies 8 doublings below it: kept at 2^-2 at least, that weight and those to 2^-4 of it have all their bits.
+constexpr float kPpFall = 8.f, kPpReach = 40.f;
 // Largest |log2 of a weight| that f32 holds to an eighth: past it the difference to the maximum, in one FMA, may pass what a first term holds.  Such rows get NaN.
 constexpr float kPpMaxScore = 1048576.f;
 constexpr uint32_t kPpGroup = 8;  // parts of an item that one CTA joins by itself

@@ -50,7 +50,7 @@ import sys
 sys.path[:0] = {path!r}
 import torch
 from test_paged_gpu import Step
-for seqs in (3046, 3047, 3071, 3072, 8192):
+for seqs in (3046, 3047, 3071, 3073, 8192):
     st = Step([5] * seqs, [1] * seqs, None, [0] * 4, 4, [[0]] * seqs, 16, seqs)
     st.run()
     torch.cuda.synchronize()
