@@ -487,11 +487,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                             nan_found = 1;
                         }
                     }
+                    if (kt == kt0) PP_WAIT(o_empty, (ni & 1) ^ 1);
+                    // (Behind that wait: it shows that the item before has had both its arrivals, so that this one counts for its own.)
                     if (kt + 1 == kt1 && lane == 0) {
                         *nan_item = (*nan_item & ~(1u << (ni & 1))) | nan_found << (ni & 1);
                         mbar_arrive(o_final);
                     }
-                    if (kt == kt0) PP_WAIT(o_empty, (ni & 1) ^ 1);
                     PP_WAIT(&p_full[pb], g / NP & 1);
                     tc_fence_after();
                     __syncwarp();

@@ -91,3 +91,22 @@ def test_lengths_that_are_cut_off_are_reported(rows):
     assert run(lambda c: c.dev.__setitem__(3, i32([90, c.width * 16 + 1]))) & 32
     assert run(lambda c: c.dev.__setitem__(2, i32([0, rows, 2 * rows + 1]))) & 32
     assert run(lambda c: c.dev.__setitem__(2, i32([0, rows, rows - 1]))) & 32
+
+
+@pytest.mark.parametrize("q_dt", [sa.BF16, sa.F16])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_row_tiles_of_one_key_tile_behind_one_another(q_dt, dim):
+    """Short prompts: every item of a CTA is one tile, and its products are under way when the next one is at hand."""
+    import torch
+
+    rng = np.random.default_rng(dim)
+    c = Case(16, 2, dim, 16, [(int(kv), int(n)) for kv, n in zip(rng.integers(5, 120, 500), rng.integers(3, 6, 500))], q_dt, sa.F32, seed=dim)
+    op = c.op()
+    c.record(op)
+    c.check()
+    first = c.out.clone()
+    for _ in range(100):
+        c.record(op)
+        torch.cuda.synchronize()
+        assert torch.equal(first, c.out)
+    assert op.device_status() == 0
