@@ -176,7 +176,9 @@ __device__ __forceinline__ void paged_share(const PagedArgs &a, uint32_t tpt, ui
             q.row0 = q.n = q.kv = 0;
             if (s < a.seqs) {
                 q = paged_seq(a, s);
-                if (blockIdx.x == 0 && pass == 1 && (a.row_starts[s + 1] > a.rows || a.row_starts[s] > a.row_starts[s + 1] || a.kv_lens[s] > a.table_stride * a.block_tokens)) atomicOr(a.words, kStatusCut);
+                if (blockIdx.x == 0 && pass == 1 && (a.row_starts[s + 1] > a.rows || a.row_starts[s] > a.row_starts[s + 1] ||
+                                                      (q.n && a.kv_lens[s] > a.table_stride * a.block_tokens)))
+                    atomicOr(a.words, kStatusCut); // (the length of a sequence without rows is not read)
                 if (q.n) cost = a.kv_heads * (per = tiles.per_head(q));
             }
             uint64_t v = cost;

@@ -89,6 +89,7 @@ def test_lengths_that_are_cut_off_are_reported(rows):
     longest = lambda c: c.dev.__setitem__(3, i32([90, c.width * 16]))  # noqa: E731 (its last pages lie outside the cache)
     assert run(longest) & 32 == 0
     assert run(lambda c: c.dev.__setitem__(3, i32([90, c.width * 16 + 1]))) & 32
+    assert run(lambda c: (c.dev.__setitem__(2, i32([0, rows, rows])), c.dev.__setitem__(3, i32([90, 1 << 30])))) == 0  # no rows: its length is not read
     assert run(lambda c: c.dev.__setitem__(2, i32([0, rows, 2 * rows + 1]))) & 32
     assert run(lambda c: c.dev.__setitem__(2, i32([0, rows, rows - 1]))) & 32
 
